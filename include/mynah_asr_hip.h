@@ -342,6 +342,112 @@ int mynah_asr_hip_aed_decode_dev(const mynah_asr_hip_aed *a, const float *enc, i
 int mynah_asr_hip_aed_forced_dev(const mynah_asr_hip_aed *a, const float *enc, int T, const int *tokens, int n,
                                  float *logits, void *stream);
 
+/* ---- a paged key-value cache for decoders that serve many sequences --------
+ * No counterpart in the reference: its decoder keeps one sequence's keys and
+ * values in two f32 arrays (src/decoder_aed.c:139-232). Here many sequences
+ * share a pool of pages; activations are f32 as everywhere in this unit, the
+ * cache f32, f16 or bf16. */
+enum {
+    MYNAH_ASR_HIP_F16 = 17,  /* cache elements (16 + their GGML type id); */
+    MYNAH_ASR_HIP_BF16 = 46  /* not weight formats */
+};
+
+/* The pool. Key (or value) of cache slot s of a page and head h: the head_dim
+ * elements at [page][h][s][0]. */
+typedef struct {
+    int type;         /* MYNAH_ASR_HIP_F32, _F16 or _BF16 */
+    int n_pages;
+    int page_size;    /* slots of a page, any number from 1 */
+    int n_kv_heads;
+    int head_dim;     /* 64 or 128 */
+    void *k, *v;      /* device, [n_pages][n_kv_heads][page_size][head_dim] each, 16-byte aligned */
+} mynah_asr_hip_kv_cache;
+
+/* The sequences of one call. Sequence b owns rows row_start[b] ..
+ * row_start[b + 1] - 1 of the activations: its newest rows. Its cache holds (for
+ * the append: will hold) len[b] keys, those rows' own among them, so row i of
+ * its n rows is at position len[b] - n + i. Key j lies in slot j % page_size of
+ * page pages[b][j / page_size]. The three tables are device memory, read when
+ * the call runs (a graph's replay reads them again); max_new and max_len bound
+ * what they hold. Whatever they hold, no call reads or writes outside its
+ * buffers: a key in a page outside [0, n_pages) is not written and not seen, nor
+ * is a key at or past max_pages * page_size; for the attention, neither is one
+ * at or past max_len, and rows of a sequence past its first max_new are left as
+ * they are. A len below 0 counts as 0. mynah_asr_hip_kv_check looks host copies
+ * over. */
+typedef struct {
+    int nseq;              /* sequences, up to 65535 */
+    int rows;              /* rows of the activation buffers, up to 2^24; those from
+                              row_start[nseq] on are left as they are */
+    int max_pages;         /* row length of `pages` */
+    int max_new;           /* most rows of one sequence */
+    int max_len;           /* most keys of one sequence, up to 2^30 */
+    const int *row_start;  /* [nseq + 1], from >= 0, not decreasing, to <= rows */
+    const int *len;        /* [nseq] */
+    const int *pages;      /* [nseq][max_pages] */
+} mynah_asr_hip_kv_batch;
+
+/* What the append does to the heads of q and k first. The norm of a head x:
+ * x / sqrt(mean(x^2) + eps) * w (squares summed in f32). Then the rotation of
+ * the first `rot` features at the row's position p: pair i becomes
+ * (a cos t - b sin t, a sin t + b cos t), t = p * freq[i] (formed in 64 bits). */
+typedef struct {
+    const float *q_norm, *k_norm;  /* device, [head_dim] each; NULL: no norm */
+    float eps;
+    int rot;                       /* features, a multiple of 8 up to head_dim; 0: no rotation */
+    int interleaved;               /* pairs (2i, 2i + 1); else (i, i + rot / 2) */
+    const double *freq;            /* device, [rot / 2], radians per position */
+} mynah_asr_hip_kv_prep;
+
+/* Norm and rotation of q and k (p; NULL: neither), q into q_out, k and v into
+ * the cache, rounded to its type to nearest even (past f16's range: infinity).
+ * q, q_out: rows of n_heads heads of head_dim floats, ldq / ldqo floats apart; k, v:
+ * rows of c->n_kv_heads heads, ldk / ldv apart (so all may lie in one buffer).
+ * n_heads 0: k and v alone (q and q_out may be NULL). q_out may be q (ldqo
+ * = ldq); no other buffers may overlap. Pointers 16-byte aligned, strides
+ * multiples of 4. Two rows for one cache slot (a page that two sequences of the
+ * call extend) race: which one stays is undefined. Uses no workspace. */
+int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b,
+                                const mynah_asr_hip_kv_prep *p, const float *q, int64_t ldq, int n_heads,
+                                float *q_out, int64_t ldqo, const float *k, int64_t ldk, const float *v, int64_t ldv,
+                                void *stream);
+
+/* Attention of the batch's rows over the cache: head h of a row sees K/V head
+ * h / (n_heads / n_kv_heads), n_heads a multiple of it,
+ *   out[h] = sum_j softmax_j(scale * q[h] . k_j) v_j
+ * over the keys j < len[b] that it sees: with causal those up to its position p;
+ * with window > 0 (causal only) of these the last `window` (itself among
+ * them) and the first `sinks` of the sequence. A row that sees no key gives 0.
+ * causal 0: every row sees all len[b] keys (cross-attention). q, out: rows of
+ * n_heads heads, ldq / ldo floats apart, 16-byte aligned, strides multiples of
+ * 4; out may be q (ldo = ldq), and may not overlap it otherwise.
+ *
+ * Products and sums as f32: |out - ref| <= 1e-5 * max|v| over the keys a row
+ * sees, for finite scores that differ by less than 2^20. A row's bits depend on
+ * its q, the keys and values it sees, its position, and the call's sizes
+ * and settings; keys and values it does not see (hidden, behind len[b], in the
+ * rest of a page) change nothing, NaN and infinity included. A row that sees a
+ * NaN or an infinity gives NaN or infinity where f32 arithmetic does, or NaN where
+ * it gives infinity.
+ *
+ * ws: device workspace of ws_bytes, 16-byte aligned, at least
+ * mynah_asr_hip_kv_attention_ws_bytes; NULL: the calling thread's own, grown as
+ * needed. Calls that may overlap in time (two streams, replays of two graphs)
+ * need a workspace each. */
+int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b, const float *q,
+                                   int64_t ldq, int n_heads, float *out, int64_t ldo, float scale, int causal,
+                                   int window, int sinks, void *ws, size_t ws_bytes, void *stream);
+/* Workspace bytes of that call, from its sizes alone (0: it needs none, or its
+ * arguments are refused; the pointers of c and b are not looked at). */
+size_t mynah_asr_hip_kv_attention_ws_bytes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b,
+                                           int n_heads, int causal, int window, int sinks);
+/* Looks over a batch whose three tables are host memory (no GPU is used; the
+ * pointers of c are not looked at): 0, or -1 and what is wrong: row_start that
+ * decreases or leaves the rows, a sequence over max_new, max_len or its pages,
+ * fewer keys than new rows, a page outside the pool, two new rows for one
+ * cache slot. */
+int mynah_asr_hip_kv_check(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b);
+
 #ifdef __cplusplus
 }
 #endif

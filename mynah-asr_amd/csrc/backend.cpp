@@ -15,11 +15,15 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "fmt.h"
+#include "kv.h"
 #include "launch.h"
 #include "mynah_asr_hip.h"
 #include "repack.h"
@@ -108,6 +112,7 @@ struct Ctx {
     DBuf enc;    // the encoder layer's activations
     DBuf ssb;    // the subsampling's activations
     DBuf gs;     // split-K GEMV workspace
+    DBuf kvw;    // paged attention's partial results
     int *pin = nullptr;   // pinned host int[2][2]: the step state of two positions read back
     hipEvent_t pev[2] = {nullptr, nullptr};   // their copies' completion
     PrepBuf pa;  // the products' input (prep_dev / qgemm_prepped_dev use this one)
@@ -1126,6 +1131,94 @@ int subsampling_dev(Ctx *c, const mynah_asr_hip_subsampling *ss, const float *fe
     return 0;
 }
 
+// ---------------------------------------------------------------------------
+// The paged key-value cache. Arguments are checked before the device is
+// looked for, so a wrong call is refused the same way everywhere.
+
+constexpr int kKvRows = 1 << 24, kKvLen = 1 << 30, kKvSeqs = 65535;
+
+int kv_type(int type) {
+    return type == MYNAH_ASR_HIP_F32 ? KV_F32 : type == MYNAH_ASR_HIP_F16 ? KV_F16 : type == MYNAH_ASR_HIP_BF16 ? KV_BF16 : -1;
+}
+
+// sizes alone (the workspace of a call depends on nothing else)
+int kv_sizes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
+    if (!c || !b) return fail("bad argument: NULL cache or batch");
+    if (kv_type(c->type) < 0) return fail("cache type must be F32, F16 or BF16");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail("head size must be 64 or 128");
+    if (c->n_pages <= 0 || c->page_size <= 0 || c->n_kv_heads <= 0) return fail("bad argument: an empty cache");
+    if ((double)c->n_pages * c->page_size * c->n_kv_heads >= 4294967295.0)
+        return fail("cache: n_pages * page_size * n_kv_heads must stay below 2^32 - 1");
+    if (b->nseq < 0 || b->nseq > kKvSeqs) return fail("batch: nseq must be 0 to 65535");
+    if (b->rows < 0 || b->rows > kKvRows) return fail("batch: rows must be 0 to 2^24");
+    if (b->max_pages < 0 || b->max_new < 0 || b->max_len < 0 || b->max_len > kKvLen)
+        return fail("batch: max_pages, max_new and max_len (up to 2^30) may not be negative");
+    return 0;
+}
+
+// buf: 16-byte aligned, rows of `width` floats `ld` apart
+int kv_rows(const char *what, const float *buf, int64_t ld, int64_t width) {
+    if (!buf) return fail("bad argument: NULL", what);
+    if ((uintptr_t)buf % 16 || ld % 4) return fail("rows must be 16-byte aligned, strides multiples of 4", what);
+    if (ld < width || ld > (int64_t)1 << 32) return fail("row stride below the row's length, or above 2^32", what);
+    return 0;
+}
+
+int kv_pointers(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
+    if (!c->k || !c->v || (uintptr_t)c->k % 16 || (uintptr_t)c->v % 16)
+        return fail("bad argument: cache buffers must be there, 16-byte aligned");
+    if (!b->row_start || !b->len || (!b->pages && b->max_pages > 0)) return fail("bad argument: a NULL table of the batch");
+    if ((uintptr_t)b->row_start % 4 || (uintptr_t)b->len % 4 || (uintptr_t)b->pages % 4)
+        return fail("bad argument: a table of the batch is not 4-byte aligned");
+    return 0;
+}
+
+// The kernels run on the current device: its stream, its memory.
+int kv_device(const void *pool, hipStream_t st) {
+    int cur = 0;
+    hipDevice_t sd = 0;
+    if (hipGetDevice(&cur) != hipSuccess) return fail("no current device");
+    if (hipStreamGetDevice(st, &sd) == hipSuccess) {
+        if ((int)sd != cur) return fail("the stream belongs to another device than the current one");
+    } else {
+        (void)hipGetLastError();
+    }
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, pool) == hipSuccess) {
+        if (at.type == hipMemoryTypeDevice && at.device != cur)
+            return fail("the cache lies on another device than the current one");
+    } else {
+        (void)hipGetLastError();
+    }
+    return 0;
+}
+
+KvTables kv_tables(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
+    return KvTables{c->k, c->v, b->row_start, b->len, b->pages, c->n_pages, c->page_size, c->n_kv_heads,
+                    b->nseq, b->rows, b->max_pages};
+}
+
+int kv_attend_sizes(const mynah_asr_hip_kv_cache *c, int n_heads, int causal, int window, int sinks) {
+    if (n_heads <= 0 || n_heads % c->n_kv_heads) return fail("n_heads must be a multiple of the cache's n_kv_heads");
+    if (n_heads > 65536) return fail("n_heads must be at most 65536");
+    if (window < 0 || sinks < 0) return fail("window and sinks may not be negative");
+    if (window > 0 && !causal) return fail("a sliding window needs causal order");
+    if (sinks > 0 && !window) return fail("first keys that stay visible need a sliding window");
+    return 0;
+}
+
+KvAttend kv_attend(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b, int n_heads, int causal, int window,
+                   int sinks) {
+    KvAttend p{};
+    p.G = n_heads / c->n_kv_heads;
+    p.max_new = std::min(b->max_new, b->rows);
+    p.max_len = b->max_len;
+    p.causal = causal != 0;
+    p.window = window > kKvLen ? 0 : window;   // (such a window hides nothing)
+    p.sinks = p.window ? std::min(sinks, kKvLen) : 0;
+    return p;
+}
+
 int begin(Ctx **c) {
     t_err[0] = 0;
     if (!mynah_asr_hip_available()) return fail("no gfx950 device");
@@ -1339,6 +1432,121 @@ int mynah_asr_hip_relpos_attention(const float *q, const float *k, const float *
     if (mynah_asr_hip_relpos_attention_dev(dq, dk, dv, drk, dbu, dbv, dctx, T, d, H, left, right, 1, c->st))
         return -1;
     return d2h_sync(c, ctx, dctx, td);
+}
+
+int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b,
+                                const mynah_asr_hip_kv_prep *p, const float *q, int64_t ldq, int n_heads,
+                                float *q_out, int64_t ldqo, const float *k, int64_t ldk, const float *v, int64_t ldv,
+                                void *stream) {
+    t_err[0] = 0;
+    if (kv_sizes(c, b) || kv_pointers(c, b)) return -1;
+    const int dk = c->head_dim;
+    if (n_heads < 0 || n_heads > 65536) return fail("n_heads must be 0 to 65536");
+    if (n_heads && (kv_rows("q", q, ldq, (int64_t)n_heads * dk) || kv_rows("q_out", q_out, ldqo, (int64_t)n_heads * dk)))
+        return -1;
+    if (kv_rows("k", k, ldk, (int64_t)c->n_kv_heads * dk) || kv_rows("v", v, ldv, (int64_t)c->n_kv_heads * dk)) return -1;
+    if (n_heads && q_out == q && ldqo != ldq) return fail("q_out may be q with the same stride alone");
+    KvAppend a{};
+    a.q = q, a.k = k, a.v = v, a.qo = q_out, a.ldq = ldq, a.ldqo = ldqo, a.ldk = ldk, a.ldv = ldv, a.Hq = n_heads;
+    if (p) {
+        if (p->rot < 0 || p->rot % 8 || p->rot > dk) return fail("rot must be a multiple of 8 up to the head size");
+        if (p->rot && (!p->freq || (uintptr_t)p->freq % 8)) return fail("a rotation needs its freq, 8-byte aligned");
+        if ((uintptr_t)p->q_norm % 16 || (uintptr_t)p->k_norm % 16) return fail("norm weights must be 16-byte aligned");
+        if ((p->q_norm || p->k_norm) && !(p->eps >= 0.0f && std::isfinite(p->eps))) return fail("eps must be finite, from 0");
+        a.qn = p->q_norm, a.kn = p->k_norm, a.eps = p->eps, a.rot = p->rot, a.inter = p->interleaved != 0;
+        a.freq = p->freq;
+    }
+    Ctx *x;
+    if (begin(&x)) return -1;
+    hipStream_t st = pick_stream(stream);
+    if (kv_device(c->k, st)) return -1;
+    if (b->rows == 0 || b->nseq == 0) return 0;
+    hipError_t e = mh_launch_kv_append(kv_tables(c, b), kv_type(c->type), dk, a, st);
+    return e == hipSuccess ? 0 : fail("append launch failed", hipGetErrorString(e));
+}
+
+size_t mynah_asr_hip_kv_attention_ws_bytes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b,
+                                           int n_heads, int causal, int window, int sinks) {
+    t_err[0] = 0;
+    if (kv_sizes(c, b) || kv_attend_sizes(c, n_heads, causal, window, sinks)) return 0;
+    if (b->nseq == 0 || b->rows == 0 || b->max_new == 0) return 0;
+    const int64_t n = mh_kv_attention_ws(b->nseq, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
+                                         c->head_dim, kv_attend(c, b, n_heads, causal, window, sinks));
+    if (n < 0) {
+        fail("attention: nseq, max_new and max_len bound too many workgroups");
+        return 0;
+    }
+    return (size_t)n * sizeof(float);
+}
+
+int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b, const float *q,
+                                   int64_t ldq, int n_heads, float *out, int64_t ldo, float scale, int causal,
+                                   int window, int sinks, void *ws, size_t ws_bytes, void *stream) {
+    t_err[0] = 0;
+    if (kv_sizes(c, b) || kv_pointers(c, b) || kv_attend_sizes(c, n_heads, causal, window, sinks)) return -1;
+    const int64_t width = (int64_t)n_heads * c->head_dim;
+    if (kv_rows("q", q, ldq, width) || kv_rows("out", out, ldo, width)) return -1;
+    if (out == q && ldo != ldq) return fail("out may be q with the same stride alone");
+    if (!std::isfinite(scale)) return fail("scale must be finite");
+    if ((uintptr_t)ws % 16) return fail("the workspace must be 16-byte aligned");
+    KvAttend p = kv_attend(c, b, n_heads, causal, window, sinks);
+    p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo, p.scale = scale;
+    size_t need = 0;
+    const bool none = b->nseq == 0 || b->rows == 0 || b->max_new == 0;
+    if (!none) {
+        const int64_t n = mh_kv_attention_ws(b->nseq, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
+                                             c->head_dim, p);
+        if (n < 0) return fail("attention: nseq, max_new and max_len bound too many workgroups");
+        need = (size_t)n * sizeof(float);
+        if (ws && ws_bytes < need) return fail("the workspace is smaller than kv_attention_ws_bytes");
+    }
+    Ctx *x;
+    if (begin(&x)) return -1;
+    hipStream_t st = pick_stream(stream);
+    if (kv_device(c->k, st)) return -1;
+    if (none) return 0;
+    if (!ws && need) {
+        note_capture(st);   // the thread's workspace may grow
+        ws = x->kvw.get(need);
+        if (!ws) return fail("workspace allocation failed");
+    }
+    hipError_t e = mh_launch_kv_attention(kv_tables(c, b), kv_type(c->type), c->head_dim, p, (float *)ws, st);
+    return e == hipSuccess ? 0 : fail("attention launch failed", hipGetErrorString(e));
+}
+
+int mynah_asr_hip_kv_check(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
+    t_err[0] = 0;
+    if (kv_sizes(c, b)) return -1;
+    if (!b->row_start || !b->len || (!b->pages && b->max_pages > 0)) return fail("bad argument: a NULL table of the batch");
+    char at[64];
+    if (b->row_start[0] < 0) return fail("row_start[0] is negative");
+    std::vector<uint64_t> slots;   // of the new rows
+    try {
+        slots.reserve((size_t)b->rows);
+    } catch (const std::bad_alloc &) {
+        return fail("out of host memory");
+    }
+    for (int s = 0; s < b->nseq; s++) {
+        snprintf(at, sizeof at, "sequence %d", s);
+        const int64_t r0 = b->row_start[s], r1 = b->row_start[s + 1], n = r1 - r0, len = b->len[s];
+        if (n < 0) return fail("row_start decreases", at);
+        if (r1 > b->rows) return fail("row_start leaves the rows", at);
+        if (n > b->max_new) return fail("more new rows than max_new", at);
+        if (len < n) return fail("fewer keys than new rows", at);
+        if (len > b->max_len) return fail("more keys than max_len", at);
+        if (len > (int64_t)b->max_pages * c->page_size) return fail("more keys than max_pages hold", at);
+        for (int64_t i = 0; i * c->page_size < len; i++) {
+            const int pg = b->pages[(size_t)s * b->max_pages + i];
+            if (pg < 0 || pg >= c->n_pages) return fail("a page outside the cache", at);
+        }
+        for (int64_t j = len - n; j < len; j++)
+            slots.push_back((uint64_t)b->pages[(size_t)s * b->max_pages + j / c->page_size] * c->page_size +
+                            j % c->page_size);
+    }
+    std::sort(slots.begin(), slots.end());
+    for (size_t i = 1; i < slots.size(); i++)
+        if (slots[i] == slots[i - 1]) return fail("two new rows for one cache slot");
+    return 0;
 }
 
 int mynah_asr_hip_encoder_layer_dev(const mynah_asr_hip_enc_layer *L, float *x, int T, int nseq, const float *pe,

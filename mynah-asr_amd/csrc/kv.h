@@ -1,0 +1,55 @@
+// kv.h — what the paged-cache kernels (kv_append.hip, kv_attention.hip) share:
+// the tables of a call, and which keys a row sees. Plain integer arithmetic,
+// for the host (workspace sizes) and the device.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#define KV_HD __host__ __device__ __forceinline__
+
+enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };   // cache elements
+
+// The pool and the tables of one call (mynah_asr_hip_kv_cache, _kv_batch).
+struct KvTables {
+    void *k, *v;
+    const int *row_start, *len, *pages;
+    int n_pages, page, Hk;        // page: slots of one
+    int nseq, rows, max_pages;
+};
+
+// One sequence: its rows r0 .. r0 + n - 1, and L keys, the rows' own among
+// them. Whatever the tables hold, 0 <= r0, r0 + n <= rows and 0 <= L <= 2^30.
+struct KvSeq {
+    int r0, n, L;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvTables &t, int b) {
+    const int r0 = max(t.row_start[b], 0), r1 = min(t.row_start[b + 1], t.rows);
+    return {r0, max(r1 - r0, 0), min(max(t.len[b], 0), 1 << 30)};
+}
+
+// Row of the pool (head_dim elements each) that holds key j of sequence b for
+// head h; KV_NONE where the table names no page of the pool. j is in [0,
+// max_pages * page). The pool's rows are fewer than 2^32 - 1 (checked on the host).
+constexpr uint32_t KV_NONE = 0xffffffffu;
+__device__ __forceinline__ uint32_t kv_slot(const KvTables &t, int b, int j, int h) {
+    const int lp = j / t.page;
+    const int pg = t.pages[(size_t)b * t.max_pages + lp];
+    return (unsigned)pg < (unsigned)t.n_pages ? ((uint32_t)pg * t.Hk + h) * t.page + (j - lp * t.page) : KV_NONE;
+}
+
+// The keys that rows between two positions see, as a list of aligned blocks of
+// KB keys: the ns blocks that the first keys lie in, then blocks first .. of
+// the window. (One run of blocks from 0 where the two meet.)
+struct KvSpan {
+    int ns, first, cnt;
+    KV_HD int block(int e) const { return e < ns ? e : first + e - ns; }
+};
+// lo: the first row's window start; hi: the last key that the last row sees (-1: none)
+template <int KB>
+KV_HD KvSpan kv_span(int lo, int hi, int sinks) {
+    const int nb = hi < 0 ? 0 : hi / KB + 1;
+    int first = lo / KB, ns = ((sinks < lo ? sinks : lo) + KB - 1) / KB;
+    if (first <= ns) first = ns = 0;
+    if (ns > nb) ns = nb;
+    return {ns, first, ns + (nb > first ? nb - first : 0)};
+}

@@ -1,0 +1,389 @@
+// kv_attention.hip — attention of new rows over a paged cache.
+//
+//   out = sum_j softmax_j(scale q . k_j) v_j over the keys j that a row sees
+//
+// with causal order, a sliding window and first keys that stay visible decided by
+// position (kv.h). The G query heads that share a K/V head are rows of one
+// product, as are a sequence's new rows: tile rows r = token * G + head, 16 a tile.
+//
+// One workgroup = four waves = one chunk of the keys that one tile sees, for one
+// K/V head. The keys are a list of blocks of 64 (kv_span); a wave takes every
+// fourth of the chunk's. It reads K and V once, from memory to registers, and
+// keeps a running maximum, sum and context of its own; the waves' are joined in
+// LDS, the chunks' by k_kv_join (a tile of one chunk is written at once). The
+// chunk's size depends on the number of blocks the tile sees alone, so a row's
+// bits do not depend on the other sequences of the call.
+//
+// Products: S^T = K Q^T and O^T = V^T P^T on the f32 MFMA 16x16x4 (lane l, c = l
+// & 15, g = l >> 4: A row c, slot g; B column c, slot g; D rows 4g + e, column c).
+// S^T leaves lane (c, g) with keys 4g + e of query row c, which is where slot g of
+// step e of the second product wants them: probabilities never leave their lane.
+// The order of features is free in both, so a lane loads runs of 16 bytes.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "kv.h"
+#include "launch.h"
+#include "product.h"
+
+namespace {
+
+constexpr int NW = 4, NTH = 64 * NW;
+constexpr int KB = 64;      // keys of a block
+constexpr int RT = 16;      // rows of a tile
+
+// Blocks a wave takes in one chunk of a tile that sees `cnt`: long lists have
+// longer chunks (fewer partial results to join).
+KV_HD int wave_blocks(int cnt) { return cnt <= 256 ? 1 : cnt <= 1024 ? 2 : 4; }
+KV_HD int chunk_blocks(int cnt) { return NW * wave_blocks(cnt); }
+KV_HD int chunks_of(int cnt) { return cnt <= 0 ? 1 : (cnt + chunk_blocks(cnt) - 1) / chunk_blocks(cnt); }
+
+// most chunks of a tile that sees up to n blocks
+int most_chunks(int n) {
+    int m = chunks_of(n);
+    if (n > 256) m = m > chunks_of(256) ? m : chunks_of(256);
+    if (n > 1024) m = m > chunks_of(1024) ? m : chunks_of(1024);
+    return m;
+}
+
+struct StepArgs {
+    KvTables t;
+    KvAttend a;
+    float *part;      // partial contexts [workgroup][R][DK], then their maxima and sums [workgroup][R][2]
+    int nrt, nch, R;  // row tiles of a sequence, chunks of a tile (at most), rows of a partial result
+};
+
+// What the rows of tile rt of a sequence see.
+struct Tile {
+    KvSeq s;
+    int live;               // rows
+    int lo0, hi0, lo1, hi1; // the first and the last row's window start and last key
+    KvSpan sp;
+};
+__device__ __forceinline__ int last_key(const KvTables &t, const KvAttend &a, const KvSeq &s, int i) {
+    const int64_t cap = (int64_t)t.max_pages * t.page;
+    const int top = (int)min((int64_t)min(s.L, a.max_len), cap) - 1;
+    return a.causal ? min(s.L - s.n + i, top) : top;
+}
+__device__ __forceinline__ int first_key(const KvAttend &a, const KvSeq &s, int i) {
+    return a.window ? max(s.L - s.n + i - a.window + 1, 0) : 0;
+}
+__device__ __forceinline__ Tile tile_of(const StepArgs &A, int b, int rt) {
+    Tile T;
+    T.s = kv_seq(A.t, b);
+    const int rows = min(T.s.n, A.a.max_new) * A.a.G;
+    T.live = min(rows - rt * RT, RT);
+    if (T.live <= 0) return T;
+    const int i0 = rt * RT / A.a.G, i1 = (rt * RT + T.live - 1) / A.a.G;
+    T.lo0 = first_key(A.a, T.s, i0);
+    T.lo1 = first_key(A.a, T.s, i1);
+    T.hi0 = last_key(A.t, A.a, T.s, i0);
+    T.hi1 = last_key(A.t, A.a, T.s, i1);
+    T.sp = kv_span<KB>(T.lo0, T.hi1, A.a.sinks);
+    return T;
+}
+
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float max_g(float x) {   // over the four lanes of a query row
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float sum_g(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+// N elements of the cache from p, as f32
+template <int N> __device__ __forceinline__ void load_run(const float *p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *(f4 *)(x + i) = *(const f4 *)(p + i);
+}
+template <int N, typename T> __device__ __forceinline__ void load_run(const T *p, float (&x)[N]) {
+    typedef T tn __attribute__((ext_vector_type(N)));
+    const tn v = *(const tn *)p;
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = (float)v[i];
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
+    constexpr int EL = 16 / sizeof(T);       // features of a 16-byte load
+    constexpr int NK = DK / (4 * EL);        // such loads of a key, per lane
+    constexpr int VE = DK / 16;              // features of a value row, per lane
+    constexpr int OS = DK + 4;
+    __shared__ uint32_t slots[NW][KB];
+    __shared__ float mls[NW][RT][2];
+    __shared__ __attribute__((aligned(16))) float os[NW][RT][OS];
+    const KvTables &t = A.t;
+    const KvAttend &a = A.a;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+    int at = blockIdx.x;
+    const int h = at % t.Hk;
+    at /= t.Hk;
+    const int ch = at % A.nch;
+    at /= A.nch;
+    const int rt = at % A.nrt, b = at / A.nrt;
+    const Tile tl = tile_of(A, b, rt);
+    if (tl.live <= 0) return;
+    const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
+    if (ch >= nch) return;
+
+    // this lane's query row, times scale and log2(e)
+    const int r = rt * RT + c, tok = min(r, rt * RT + tl.live - 1) / a.G;
+    const int lo = first_key(a, tl.s, tok), hi = last_key(t, a, tl.s, tok);
+    float q[NK][EL];
+    {
+        const float *qp = a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK;
+        const float f = a.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            if (c < tl.live) load_run<EL>(qp + 4 * EL * i + EL * g, q[i]);
+#pragma unroll
+            for (int e = 0; e < EL; e++) q[i][e] = c < tl.live ? q[i][e] * f : 0.0f;
+        }
+    }
+    float m = -INFINITY, l = 0.0f;
+    f4 o[VE];
+#pragma unroll
+    for (int e = 0; e < VE; e++) o[e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int e1 = min(e0 + chunk_blocks(tl.sp.cnt), tl.sp.cnt);
+    for (int e = e0 + w; e < e1; e += NW) {
+        const int j0 = tl.sp.block(e) * KB;
+        // where the block's keys lie; `all`: every row sees every one of them
+        const int jl = j0 + lane;
+        const uint32_t at_l = jl <= tl.hi1 ? kv_slot(t, b, jl, h) : KV_NONE;
+        const bool all = __all(at_l != KV_NONE && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks));
+        wave_lds_order();   // the reads of the last block's slots
+        slots[w][lane] = at_l;
+        wave_lds_order();
+        f4 s[KB / 16];
+#pragma unroll
+        for (int n = 0; n < KB / 16; n++) {
+            const uint32_t at_k = slots[w][16 * n + c];
+            const T *kp = (const T *)t.k + (size_t)(at_k == KV_NONE ? 0 : at_k) * DK;
+            s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                float k[EL];
+                load_run<EL>(kp + 4 * EL * i + EL * g, k);
+#pragma unroll
+                for (int x = 0; x < EL; x++) s[n] = mfma4(k[x], q[i][x], s[n]);
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < KB / 16; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int jj = 16 * n + 4 * g + x, j = j0 + jj;
+                if (!all) {
+                    const bool see = slots[w][jj] != KV_NONE && j <= hi && (j >= lo || j < a.sinks);
+                    s[n][x] = see ? s[n][x] : -INFINITY;
+                }
+                mx = fmaxf(mx, s[n][x]);
+            }
+        const float mn = fmaxf(m, max_g(mx)), mz = mn == -INFINITY ? 0.0f : mn;
+        const float al = exp2f(m - mz);
+        m = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < KB / 16; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                s[n][x] = exp2f(s[n][x] - mz);
+                sum += s[n][x];
+            }
+        l = l * al + sum;
+#pragma unroll
+        for (int x = 0; x < VE; x++) o[x] *= al;
+        // Values. A key that only some rows see meets the others' probability 0,
+        // which hides it unless it is not finite: such an element counts as 0 in
+        // the product and is added to the rows that see it afterwards.
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < KB / 16; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int jj = 16 * n + 4 * g + x;
+                const uint32_t at_v = slots[w][jj];
+                float v[VE];
+                load_run<VE>((const T *)t.v + (size_t)(at_v == KV_NONE ? 0 : at_v) * DK + VE * c, v);
+                if (!all) {
+#pragma unroll
+                    for (int y = 0; y < VE; y++) {
+                        const bool fin = fabsf(v[y]) < INFINITY;
+                        odd = odd || (!fin && at_v != KV_NONE);
+                        v[y] = fin && at_v != KV_NONE ? v[y] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < VE; y++) o[y] = mfma4(v[y], s[n][x], o[y]);
+            }
+        if (__any(odd)) {
+            for (int jj = 0; jj < KB; jj++) {
+                const uint32_t at_v = slots[w][jj];
+                const int j = j0 + jj;
+                if (at_v == KV_NONE || j > hi || (j < lo && j >= a.sinks)) continue;
+                const T *vp = (const T *)t.v + (size_t)at_v * DK;
+                for (int x = 0; x < 4; x++)
+                    for (int y = 0; y < VE; y++) {
+                        const float v = (float)vp[VE * (4 * g + x) + y];
+                        if (!(fabsf(v) < INFINITY)) o[y][x] += v;
+                    }
+            }
+        }
+    }
+    l = sum_g(l);
+
+    // join the waves
+    if (g == 0) mls[w][c][0] = m, mls[w][c][1] = l;
+    __syncthreads();
+    float mb = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NW; i++) mb = fmaxf(mb, mls[i][c][0]);
+    const float mz = mb == -INFINITY ? 0.0f : mb, f = exp2f(m - mz);
+    float lb = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; i++) lb += mls[i][c][1] * exp2f(mls[i][c][0] - mz);
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int y = 0; y < VE; y += 4) {
+            f4 u;
+#pragma unroll
+            for (int z = 0; z < 4; z++) u[z] = o[y + z][x] * f;
+            *(f4 *)(&os[w][c][VE * (4 * g + x) + y]) = u;
+        }
+    if (w == 0 && g == 0 && nch > 1 && c < tl.live) {
+        float *ml = A.part + (size_t)gridDim.x * A.R * DK + ((size_t)blockIdx.x * A.R + c) * 2;
+        ml[0] = mb;
+        ml[1] = lb;
+    }
+    __syncthreads();
+    for (int i = tid; i < tl.live * (DK / 4); i += NTH) {
+        const int row = i / (DK / 4), d = 4 * (i % (DK / 4));
+        f4 u = *(const f4 *)&os[0][row][d];
+#pragma unroll
+        for (int k = 1; k < NW; k++) u += *(const f4 *)&os[k][row][d];
+        if (nch > 1) {
+            *(f4 *)(A.part + ((size_t)blockIdx.x * A.R + row) * DK + d) = u;
+            continue;
+        }
+        float ms = -INFINITY, ls = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; k++) ms = fmaxf(ms, mls[k][row][0]);
+        ms = ms == -INFINITY ? 0.0f : ms;
+#pragma unroll
+        for (int k = 0; k < NW; k++) ls += mls[k][row][1] * exp2f(mls[k][row][0] - ms);
+        const int rr = rt * RT + row;
+        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+        *(f4 *)(a.out + (int64_t)(tl.s.r0 + rr / a.G) * a.ldo + (h * a.G + rr % a.G) * DK + d) = u * inv;
+    }
+}
+
+// The chunks of a row, joined in their order: out = sum_c 2^(m_c - M) O_c / sum_c
+// 2^(m_c - M) l_c. One workgroup a row and K/V head; NG groups of lanes take every
+// NG-th chunk, then the groups are added in order.
+template <int DK>
+__global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
+    constexpr int LN = DK / 4, NG = NTH / LN;
+    __shared__ float red[NW];
+    __shared__ __attribute__((aligned(16))) float os[NG][DK];
+    __shared__ float ls[NG];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.y;
+    int at = blockIdx.x;
+    const int h = at % A.t.Hk;
+    at /= A.t.Hk;
+    const int rt = at % A.nrt, b = at / A.nrt;
+    const Tile tl = tile_of(A, b, rt);
+    if (row >= tl.live) return;
+    const int nch = chunks_of(tl.sp.cnt);
+    if (nch <= 1) return;
+    // chunk i's workgroup: ((b nrt + rt) nch_max + i) Hk + h
+    const size_t wg0 = ((size_t)b * A.nrt + rt) * A.nch * A.t.Hk + h;
+    const size_t wgs = (size_t)A.t.nseq * A.nrt * A.nch * A.t.Hk;
+    const float *ml = A.part + wgs * A.R * DK;
+    auto slot = [&](int i) { return (wg0 + (size_t)i * A.t.Hk) * A.R + row; };
+    float m = -INFINITY;
+    for (int i = tid; i < nch; i += NTH) m = fmaxf(m, ml[2 * slot(i)]);
+    m = wave_max<64>(m);
+    if (lane == 0) red[w] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float mz = m == -INFINITY ? 0.0f : m;
+    const int gi = tid / LN, d = 4 * (tid % LN);
+    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int i = gi; i < nch; i += NG) {
+        const size_t s = slot(i);
+        const float f = exp2f(ml[2 * s] - mz);
+        l += f * ml[2 * s + 1];
+        o += f * *(const f4 *)(A.part + s * DK + d);
+    }
+    *(f4 *)&os[gi][d] = o;
+    if (d == 0) ls[gi] = l;
+    __syncthreads();
+    if (gi == 0) {
+#pragma unroll
+        for (int i = 1; i < NG; i++) {
+            o += *(const f4 *)&os[i][d];
+            l += ls[i];
+        }
+        const int rr = rt * RT + row;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *(f4 *)(A.a.out + (int64_t)(tl.s.r0 + rr / A.a.G) * A.a.ldo + (h * A.a.G + rr % A.a.G) * DK + d) = o * inv;
+    }
+}
+
+// The launch's sizes: row tiles of a sequence, chunks of a tile, rows of a partial result.
+struct Plan {
+    int nrt, nch, R;
+    int64_t wgs;
+};
+Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
+    Plan p;
+    const int64_t rows = (int64_t)a.max_new * a.G;
+    p.nrt = (int)((rows + RT - 1) / RT);
+    p.R = rows < RT ? (int)rows : RT;
+    const int64_t cap = (int64_t)max_pages * page;
+    const int keys = (int)(a.max_len < cap ? a.max_len : cap), all = (keys + KB - 1) / KB;
+    int64_t blocks = all;
+    if (a.window) {
+        // a tile's rows are up to ceil(16 / G) tokens apart; each end of each part may cut a block
+        const int64_t toks = (RT + a.G - 1) / a.G + 1;
+        const int64_t win = ((int64_t)a.window + toks + KB - 1) / KB + 1, sink = ((int64_t)a.sinks + KB - 1) / KB + 1;
+        if (win + sink < blocks) blocks = win + sink;
+    }
+    p.nch = most_chunks((int)blocks);
+    p.wgs = (int64_t)nseq * p.nrt * p.nch * Hk;
+    return p;
+}
+
+}  // namespace
+
+int64_t mh_kv_attention_ws(int nseq, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
+    if ((int64_t)a.max_new * a.G >= 1 << 30) return -1;
+    const Plan p = plan_of(nseq, Hk, page, max_pages, a);
+    if (p.wgs >= 1 << 30) return -1;
+    return p.nch > 1 ? p.wgs * p.R * (dk + 2) : 0;
+}
+
+hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
+    const Plan p = plan_of(t.nseq, t.Hk, t.page, t.max_pages, a);
+    const StepArgs A{t, a, ws, p.nrt, p.nch, p.R};
+    auto go = [&](auto step, auto join) {
+        hipLaunchKernelGGL(step, dim3((unsigned)p.wgs), dim3(NTH), 0, st, A);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.nch <= 1) return e;
+        hipLaunchKernelGGL(join, dim3((unsigned)((int64_t)t.nseq * p.nrt * t.Hk), p.R), dim3(NTH), 0, st, A);
+        return hipGetLastError();
+    };
+    if (dk == 128)
+        return type == KV_F32 ? go(k_kv_step<float, 128>, k_kv_join<128>)
+               : type == KV_F16 ? go(k_kv_step<_Float16, 128>, k_kv_join<128>)
+                                : go(k_kv_step<__bf16, 128>, k_kv_join<128>);
+    return type == KV_F32 ? go(k_kv_step<float, 64>, k_kv_join<64>)
+           : type == KV_F16 ? go(k_kv_step<_Float16, 64>, k_kv_join<64>)
+                            : go(k_kv_step<__bf16, 64>, k_kv_join<64>);
+}

@@ -210,3 +210,29 @@ struct MhEmbNext {
 hipError_t mh_launch_argmax(const float *logits, int vocab, int *st, const MhEmbNext &en, hipStream_t s);
 hipError_t mh_launch_bias_rows(float *y, const float *b, size_t rows, int d, hipStream_t s);
 hipError_t mh_launch_set_state(int *st, int p, int cur, hipStream_t s);
+
+// The paged key-value cache (kv_append.hip, kv_attention.hip; tables: kv.h)
+struct KvTables;
+struct KvAppend {
+    const float *q, *k, *v;
+    float *qo;
+    int64_t ldq, ldqo, ldk, ldv;
+    const float *qn, *kn;   // or null: no norm
+    const double *freq;
+    float eps;
+    int Hq, rot, inter;
+};
+// type: KV_F32, _F16 or _BF16; dk 64 or 128. rows > 0.
+hipError_t mh_launch_kv_append(const KvTables &t, int type, int dk, const KvAppend &p, hipStream_t st);
+struct KvAttend {
+    const float *q;
+    float *out;
+    int64_t ldq, ldo;
+    int G;                  // query heads of a K/V head
+    int max_new, max_len;
+    float scale;
+    int causal, window, sinks;   // window 0: none
+};
+// Workspace floats of the call below (0: none; < 0: too many workgroups)
+int64_t mh_kv_attention_ws(int nseq, int Hk, int page, int max_pages, int type, int dk, const KvAttend &p);
+hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &p, float *ws, hipStream_t st);

@@ -27,6 +27,7 @@ NAMES = {F32: "F32", INT8: "INT8", INT4: "INT4", Q4_0: "Q4_0", Q8_0: "Q8_0", Q2_
 BITS = {F32: 32.0, INT8: 8.0, INT4: 5.0, Q4_0: 4.5, Q8_0: 8.5, Q2_K: 2.625, Q3_K: 3.4375,
         Q4_K: 4.5, Q5_K: 5.5, Q6_K: 6.5625}
 EXACT, INT8ACT, QMAT = 0, 1, 2
+F16, BF16 = 17, 46   # element types of a paged cache, with F32
 
 # every symbol include/mynah_asr_hip.h declares
 HIP_SYMBOLS = [
@@ -41,6 +42,8 @@ HIP_SYMBOLS = [
     "mynah_asr_hip_aed_decode_dev", "mynah_asr_hip_aed_forced_dev",
     "mynah_asr_hip_qgemm_noalloc_dev", "mynah_asr_hip_noalloc_bytes", "mynah_asr_hip_read_floor_dev",
     "mynah_asr_hip_encoder_layer_dev", "mynah_asr_hip_subsampling_dev",
+    "mynah_asr_hip_kv_append_dev", "mynah_asr_hip_kv_attention_dev", "mynah_asr_hip_kv_attention_ws_bytes",
+    "mynah_asr_hip_kv_check",
 ]
 HOST_SYMBOLS = [
     "mynah_asr_set_backend", "mynah_asr_backend", "mynah_asr_gemm_wt", "mynah_asr_silu",
@@ -87,6 +90,24 @@ class SubsamplingC(C.Structure):
                 ("dw_b", C.c_void_p * 2), ("pw_w", C.c_void_p * 2), ("pw_b", C.c_void_p * 2),
                 ("lin_w", C.c_void_p), ("lin_b", C.c_void_p), ("channels", C.c_int), ("d_model", C.c_int),
                 ("causal", C.c_int)]
+
+
+class KvCacheC(C.Structure):
+    """mynah_asr_hip_kv_cache (include/mynah_asr_hip.h)."""
+    _fields_ = [("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class KvBatchC(C.Structure):
+    """mynah_asr_hip_kv_batch (include/mynah_asr_hip.h)."""
+    _fields_ = [("nseq", C.c_int), ("rows", C.c_int), ("max_pages", C.c_int), ("max_new", C.c_int),
+                ("max_len", C.c_int), ("row_start", C.c_void_p), ("len", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class KvPrepC(C.Structure):
+    """mynah_asr_hip_kv_prep (include/mynah_asr_hip.h)."""
+    _fields_ = [("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rot", C.c_int),
+                ("interleaved", C.c_int), ("freq", C.c_void_p)]
 
 
 class WDesc(C.Structure):
@@ -163,6 +184,15 @@ class HipLib:
             L.mynah_asr_hip_aed_decode_dev.argtypes = [C.POINTER(AedC), _P, C.c_int, _P, C.c_int, C.c_int, _P,
                                                        C.c_int, _P]
             L.mynah_asr_hip_aed_forced_dev.argtypes = [C.POINTER(AedC), _P, C.c_int, _P, C.c_int, _P, _P]
+        if hasattr(L, "mynah_asr_hip_kv_append_dev"):
+            kv = [C.POINTER(KvCacheC), C.POINTER(KvBatchC)]
+            L.mynah_asr_hip_kv_append_dev.argtypes = kv + [C.POINTER(KvPrepC), _P, C.c_int64, C.c_int, _P, C.c_int64, _P,
+                                                           C.c_int64, _P, C.c_int64, _P]
+            L.mynah_asr_hip_kv_attention_dev.argtypes = kv + [_P, C.c_int64, C.c_int, _P, C.c_int64, C.c_float] + \
+                [C.c_int] * 3 + [_P, C.c_size_t, _P]
+            L.mynah_asr_hip_kv_attention_ws_bytes.restype = C.c_size_t
+            L.mynah_asr_hip_kv_attention_ws_bytes.argtypes = kv + [C.c_int] * 4
+            L.mynah_asr_hip_kv_check.argtypes = kv
         L.mynah_asr_hip_qgemm.argtypes = [C.POINTER(WDesc), _P, _P, C.c_int]
         L.mynah_asr_hip_qffn.argtypes = [C.POINTER(WDesc), C.POINTER(WDesc), _P, _P, C.c_int]
         L.mynah_asr_hip_qqkv.argtypes = [C.POINTER(WDesc)] * 3 + [_P] * 4 + [C.c_int]
@@ -354,6 +384,53 @@ def host_relpos_attention(lib, q, k, v, rk, bias_u, bias_v, H: int, left: int = 
                                              _ptr(ctx), T, d, H, left, right)
     lib._check(rc, "relpos_attention")
     return ctx
+
+
+def kv_cache(type: int, k: int, v: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> KvCacheC:
+    """A paged cache's pool (mynah_asr_hip_kv_cache): type F32, F16 or BF16; k, v device pointers of
+    [n_pages, n_kv_heads, page_size, head_dim]."""
+    return KvCacheC(type, n_pages, page_size, n_kv_heads, head_dim, k, v)
+
+
+def kv_batch(row_start: int, len: int, pages: int, nseq: int, rows: int, max_pages: int, max_new: int,
+             max_len: int) -> KvBatchC:
+    """The sequences of a call (mynah_asr_hip_kv_batch): row_start [nseq + 1], len [nseq] and pages
+    [nseq, max_pages] are device pointers of int32 (host pointers for kv_check)."""
+    return KvBatchC(nseq, rows, max_pages, max_new, max_len, row_start, len, pages)
+
+
+def kv_prep(q_norm: int | None = None, k_norm: int | None = None, eps: float = 1e-6, rot: int = 0,
+            interleaved: bool = False, freq: int | None = None) -> KvPrepC:
+    """Head norms and rotation of an append (mynah_asr_hip_kv_prep); freq: a device pointer of rot / 2 doubles."""
+    return KvPrepC(q_norm, k_norm, eps, rot, int(interleaved), freq)
+
+
+def kv_append_dev(lib, cache: KvCacheC, batch: KvBatchC, prep: KvPrepC | None, q, ldq: int, n_heads: int, q_out,
+                  ldqo: int, k, ldk: int, v, ldv: int, stream: int = 0):
+    """q normed and rotated into q_out, k (the same) and v into the cache (mynah_asr_hip_kv_append_dev)."""
+    rc = lib.L.mynah_asr_hip_kv_append_dev(cache, batch, prep, q, ldq, n_heads, q_out, ldqo, k, ldk, v, ldv,
+                                           stream or None)
+    lib._check(rc, "kv_append_dev")
+
+
+def kv_attention_dev(lib, cache: KvCacheC, batch: KvBatchC, q, ldq: int, n_heads: int, out, ldo: int, scale: float,
+                     causal: int = 1, window: int = 0, sinks: int = 0, ws: int = 0, ws_bytes: int = 0,
+                     stream: int = 0):
+    """Attention of the batch's rows over the cache (mynah_asr_hip_kv_attention_dev)."""
+    rc = lib.L.mynah_asr_hip_kv_attention_dev(cache, batch, q, ldq, n_heads, out, ldo, scale, causal, window, sinks,
+                                              ws or None, ws_bytes, stream or None)
+    lib._check(rc, "kv_attention_dev")
+
+
+def kv_attention_ws_bytes(lib, cache: KvCacheC, batch: KvBatchC, n_heads: int, causal: int = 1, window: int = 0,
+                          sinks: int = 0) -> int:
+    """Workspace bytes of such a call (mynah_asr_hip_kv_attention_ws_bytes)."""
+    return int(lib.L.mynah_asr_hip_kv_attention_ws_bytes(cache, batch, n_heads, causal, window, sinks))
+
+
+def kv_check(lib, cache: KvCacheC, batch: KvBatchC) -> None:
+    """Looks over a batch of host tables (mynah_asr_hip_kv_check); raises with what is wrong."""
+    lib._check(lib.L.mynah_asr_hip_kv_check(cache, batch), "kv_check")
 
 
 class Gguf:
