@@ -1470,7 +1470,7 @@ size_t mynah_asr_hip_kv_attention_ws_bytes(const mynah_asr_hip_kv_cache *c, cons
     t_err[0] = 0;
     if (kv_sizes(c, b) || kv_attend_sizes(c, n_heads, causal, window, sinks)) return 0;
     if (b->nseq == 0 || b->rows == 0 || b->max_new == 0) return 0;
-    const int64_t n = mh_kv_attention_ws(b->nseq, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
+    const int64_t n = mh_kv_attention_ws(b->nseq, b->rows, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
                                          c->head_dim, kv_attend(c, b, n_heads, causal, window, sinks));
     if (n < 0) {
         fail("attention: nseq, max_new and max_len bound too many workgroups");
@@ -1494,7 +1494,7 @@ int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_
     size_t need = 0;
     const bool none = b->nseq == 0 || b->rows == 0 || b->max_new == 0;
     if (!none) {
-        const int64_t n = mh_kv_attention_ws(b->nseq, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
+        const int64_t n = mh_kv_attention_ws(b->nseq, b->rows, c->n_kv_heads, c->page_size, b->max_pages, kv_type(c->type),
                                              c->head_dim, p);
         if (n < 0) return fail("attention: nseq, max_new and max_len bound too many workgroups");
         need = (size_t)n * sizeof(float);

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "launch.h"
+
 #define KV_HD __host__ __device__ __forceinline__
 
 enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };   // cache elements
@@ -52,4 +54,37 @@ KV_HD KvSpan kv_span(int lo, int hi, int sinks) {
     if (first <= ns) first = ns = 0;
     if (ns > nb) ns = nb;
     return {ns, first, ns + (nb > first ? nb - first : 0)};
+}
+
+// What a tile of a sequence's rows sees. Rows are (token, query head of the K/V
+// head): row r is head r % G of token r / G, tile rt holds RT of them.
+struct KvTile {
+    KvSeq s;
+    int live;                 // its rows; <= 0: none, and the rest is not set
+    int lo0, hi0, lo1, hi1;   // the first and the last row's window start and last key
+    KvSpan sp;
+};
+__device__ __forceinline__ int kv_last(const KvTables &t, const KvAttend &a, const KvSeq &s, int tok) {
+    const int64_t cap = (int64_t)t.max_pages * t.page;
+    const int top = (int)min((int64_t)min(s.L, a.max_len), cap) - 1;
+    return a.causal ? min(s.L - s.n + tok, top) : top;
+}
+__device__ __forceinline__ int kv_first(const KvAttend &a, const KvSeq &s, int tok) {
+    return a.window ? max(s.L - s.n + tok - a.window + 1, 0) : 0;
+}
+// a sequence's rows that are computed
+__device__ __forceinline__ int kv_rows(const KvAttend &a, const KvSeq &s) { return min(s.n, a.max_new) * a.G; }
+template <int RT, int KB>
+__device__ __forceinline__ KvTile kv_tile(const KvTables &t, const KvAttend &a, int b, int rt) {
+    KvTile T;
+    T.s = kv_seq(t, b);
+    T.live = min(kv_rows(a, T.s) - rt * RT, RT);
+    if (T.live <= 0) return T;
+    const int i0 = rt * RT / a.G, i1 = (rt * RT + T.live - 1) / a.G;
+    T.lo0 = kv_first(a, T.s, i0);
+    T.lo1 = kv_first(a, T.s, i1);
+    T.hi0 = kv_last(t, a, T.s, i0);
+    T.hi1 = kv_last(t, a, T.s, i1);
+    T.sp = kv_span<KB>(T.lo0, T.hi1, a.sinks);
+    return T;
 }

@@ -53,36 +53,6 @@ struct StepArgs {
     int nrt, nch, R;  // row tiles of a sequence, chunks of a tile (at most), rows of a partial result
 };
 
-// What the rows of tile rt of a sequence see.
-struct Tile {
-    KvSeq s;
-    int live;               // rows
-    int lo0, hi0, lo1, hi1; // the first and the last row's window start and last key
-    KvSpan sp;
-};
-__device__ __forceinline__ int last_key(const KvTables &t, const KvAttend &a, const KvSeq &s, int i) {
-    const int64_t cap = (int64_t)t.max_pages * t.page;
-    const int top = (int)min((int64_t)min(s.L, a.max_len), cap) - 1;
-    return a.causal ? min(s.L - s.n + i, top) : top;
-}
-__device__ __forceinline__ int first_key(const KvAttend &a, const KvSeq &s, int i) {
-    return a.window ? max(s.L - s.n + i - a.window + 1, 0) : 0;
-}
-__device__ __forceinline__ Tile tile_of(const StepArgs &A, int b, int rt) {
-    Tile T;
-    T.s = kv_seq(A.t, b);
-    const int rows = min(T.s.n, A.a.max_new) * A.a.G;
-    T.live = min(rows - rt * RT, RT);
-    if (T.live <= 0) return T;
-    const int i0 = rt * RT / A.a.G, i1 = (rt * RT + T.live - 1) / A.a.G;
-    T.lo0 = first_key(A.a, T.s, i0);
-    T.lo1 = first_key(A.a, T.s, i1);
-    T.hi0 = last_key(A.t, A.a, T.s, i0);
-    T.hi1 = last_key(A.t, A.a, T.s, i1);
-    T.sp = kv_span<KB>(T.lo0, T.hi1, A.a.sinks);
-    return T;
-}
-
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float max_g(float x) {   // over the four lanes of a query row
     x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -123,14 +93,14 @@ __global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
     const int ch = at % A.nch;
     at /= A.nch;
     const int rt = at % A.nrt, b = at / A.nrt;
-    const Tile tl = tile_of(A, b, rt);
+    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
     if (tl.live <= 0) return;
     const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
     if (ch >= nch) return;
 
     // this lane's query row, times scale and log2(e)
     const int r = rt * RT + c, tok = min(r, rt * RT + tl.live - 1) / a.G;
-    const int lo = first_key(a, tl.s, tok), hi = last_key(t, a, tl.s, tok);
+    const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
     float q[NK][EL];
     {
         const float *qp = a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK;
@@ -296,7 +266,7 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
     const int h = at % A.t.Hk;
     at /= A.t.Hk;
     const int rt = at % A.nrt, b = at / A.nrt;
-    const Tile tl = tile_of(A, b, rt);
+    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
     if (row >= tl.live) return;
     const int nch = chunks_of(tl.sp.cnt);
     if (nch <= 1) return;
@@ -362,14 +332,16 @@ Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
 
 }  // namespace
 
-int64_t mh_kv_attention_ws(int nseq, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
+int64_t mh_kv_attention_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     if ((int64_t)a.max_new * a.G >= 1 << 30) return -1;
+    if (mh_kv_prompt(type, a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, dk, a);
     const Plan p = plan_of(nseq, Hk, page, max_pages, a);
     if (p.wgs >= 1 << 30) return -1;
     return p.nch > 1 ? p.wgs * p.R * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
+    if (mh_kv_prompt(type, a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
     const Plan p = plan_of(t.nseq, t.Hk, t.page, t.max_pages, a);
     const StepArgs A{t, a, ws, p.nrt, p.nch, p.R};
     auto go = [&](auto step, auto join) {

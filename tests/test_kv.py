@@ -76,7 +76,7 @@ def test_attention_refuses_small_workspace(lib):
 
 
 def test_attention_refuses_too_many_workgroups(lib):
-    b = batch(nseq=65535, rows=2 ** 24, max_new=2 ** 24, max_pages=2 ** 26, max_len=2 ** 30)
+    b = batch(nseq=65535, rows=2 ** 24, max_new=32, max_pages=2 ** 26, max_len=2 ** 30)
     refused(attention, lib, None, b)
     assert M.kv_attention_ws_bytes(lib, cache(), b, 4) == 0
 
