@@ -14,15 +14,18 @@
 // chunk's size depends on the number of blocks the tile sees alone, so a row's
 // bits do not depend on the other sequences of the call.
 //
-// Products: S^T = K Q^T and O^T = V^T P^T on the f32 MFMA 16x16x4 (lane l, c = l
-// & 15, g = l >> 4: A row c, slot g; B column c, slot g; D rows 4g + e, column c).
-// S^T leaves lane (c, g) with keys 4g + e of query row c, which is where slot g of
-// step e of the second product wants them: probabilities never leave their lane.
-// The order of features is free in both, so a lane loads runs of 16 bytes.
+// Products: S^T = K Q^T and O^T = V^T P^T (lane l, c = l & 15, g = l >> 4: A row
+// c, B column c, D rows 4g + e, column c). f32 caches: the f32 MFMA 16x16x4, slot g;
+// 16-bit ones: the 16x16x32 MFMA of their type, slots 8g + j, on q and probabilities
+// in terms (kv_terms.h). S^T leaves lane (c, g) with keys 4g + e of query row c, and
+// the second product is free to take its keys in that order: probabilities never
+// leave their lane. It is free in the order of features too, so a lane loads runs of
+// 16 bytes of a value row, and pairs the rows' elements by byte permutes.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
 #include "kv.h"
+#include "kv_terms.h"
 #include "launch.h"
 #include "product.h"
 
@@ -63,30 +66,140 @@ __device__ __forceinline__ float sum_g(float x) {
     return x + __shfl_xor(x, 32, 64);
 }
 
-// N elements of the cache from p, as f32
-template <int N> __device__ __forceinline__ void load_run(const float *p, float (&x)[N]) {
+// BYTES from p
+template <int BYTES> __device__ __forceinline__ void load_run(const void *p, uint32_t (&x)[BYTES / 4]) {
+    if constexpr (BYTES % 16 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) *(f4 *)(x + i) = *(const f4 *)(p + i);
-}
-template <int N, typename T> __device__ __forceinline__ void load_run(const T *p, float (&x)[N]) {
-    typedef T tn __attribute__((ext_vector_type(N)));
-    const tn v = *(const tn *)p;
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = (float)v[i];
+        for (int i = 0; i < BYTES / 16; i++) {
+            const uint4 v = ((const uint4 *)p)[i];
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+    } else {
+        const uint2 v = *(const uint2 *)p;
+        x[0] = v.x, x[1] = v.y;
+    }
 }
 
+// The two products of a wave on one kind of cache. Both take and give the f32
+// scores s[tile of 16 keys], keys 4 g + e of query row c in lane (c, g).
+template <typename T, int DK> struct Wave {   // 16 bits
+    using X = KvTerms<T>;
+    typedef typename X::v8 v8;
+    static constexpr int NB = KB / 16;             // key tiles at a time
+    static constexpr int NU = DK / 32, VE = DK / 16;
+    static constexpr float TOP = X::N == 2 ? 14.0f : 0.0f;   // probabilities reach 2^TOP
+    v8 q[NU][X::N];
+    float sc;
+    __device__ __forceinline__ void set_q(const float *qp, float f, bool live, int g) {
+        float x[NU][8], mx = 0.0f;
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            *(f4 *)&x[u][0] = *(const f4 *)(qp + 32 * u + 8 * g);
+            *(f4 *)&x[u][4] = *(const f4 *)(qp + 32 * u + 8 * g + 4);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[u][j] = live ? x[u][j] * f : 0.0f;
+                mx = fmaxf(mx, fabsf(x[u][j]));
+            }
+        }
+        const int e = X::shift(max_g(mx));
+        sc = ldexpf(1.0f, -e);
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[u][j] = ldexpf(x[u][j], e);
+            X::split(x[u], q[u]);
+        }
+    }
+    __device__ __forceinline__ f4 scores(const uint32_t (&k)[NU][4]) const {
+        f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const v8 kv = __builtin_bit_cast(v8, uint4{k[u][0], k[u][1], k[u][2], k[u][3]});
+#pragma unroll
+            for (int x = 0; x < X::N; x++) s = X::mfma16(kv, q[u][x], s);
+        }
+        return s * sc;
+    }
+    // o[e] += V^T P^T: feature VE (4 g + x) + e of the context in element x
+    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE / 2], const f4 (&p)[NB], f4 (&o)[VE]) {
+#pragma unroll
+        for (int n = 0; n < NB; n += 2) {
+            // slots 8 g + j: keys 4 g + j of tile n, then of tile n + 1
+            const float pf[8] = {p[n][0], p[n][1], p[n][2], p[n][3], p[n + 1][0], p[n + 1][1], p[n + 1][2], p[n + 1][3]};
+            v8 pt[X::N];
+            X::split(pf, pt);
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                uint32_t a[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int i = n + y / 2, r = 2 * (y & 1);
+                    a[y] = __builtin_amdgcn_perm(v[i][r + 1][e / 2], v[i][r][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+                }
+                const v8 av = __builtin_bit_cast(v8, uint4{a[0], a[1], a[2], a[3]});
+#pragma unroll
+                for (int x = 0; x < X::N; x++) o[e] = X::mfma16(av, pt[x], o[e]);
+            }
+        }
+    }
+    // the elements that are not finite, set to 0; whether there are any
+    static __device__ __forceinline__ bool clean(uint32_t &x) {
+        const bool l = kv_odd_lo<T>(x), h = kv_odd_hi<T>(x);
+        x = (l ? 0u : x & 0xffffu) | (h ? 0u : x & 0xffff0000u);
+        return l || h;
+    }
+};
+template <int DK> struct Wave<float, DK> {
+    static constexpr int NB = 2;                   // (twice the registers of 16 bits)
+    static constexpr int NU = DK / 16, VE = DK / 16;
+    static constexpr float TOP = 0.0f;
+    float q[NU][4];
+    __device__ __forceinline__ void set_q(const float *qp, float f, bool live, int g) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const f4 x = *(const f4 *)(qp + 16 * u + 4 * g);
+#pragma unroll
+            for (int j = 0; j < 4; j++) q[u][j] = live ? x[j] * f : 0.0f;
+        }
+    }
+    __device__ __forceinline__ f4 scores(const uint32_t (&k)[NU][4]) const {
+        f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s = mfma4(__uint_as_float(k[u][j]), q[u][j], s);
+        return s;
+    }
+    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE], const f4 (&p)[NB], f4 (&o)[VE]) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) o[e] = mfma4(__uint_as_float(v[n][x][e]), p[n][x], o[e]);
+    }
+    static __device__ __forceinline__ bool clean(uint32_t &x) {
+        const bool odd = !(fabsf(__uint_as_float(x)) < INFINITY);
+        x = odd ? 0u : x;
+        return odd;
+    }
+};
+
 template <typename T, int DK>
-__global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
+__global__ __launch_bounds__(NTH, 2) void k_kv_step(const StepArgs A) {
+    using W = Wave<T, DK>;
     constexpr int EL = 16 / sizeof(T);       // features of a 16-byte load
-    constexpr int NK = DK / (4 * EL);        // such loads of a key, per lane
-    constexpr int VE = DK / 16;              // features of a value row, per lane
+    constexpr int NB = W::NB, NU = W::NU, VE = W::VE;
+    constexpr int VB = VE * sizeof(T);       // bytes of a value row, per lane
     constexpr int OS = DK + 4;
     __shared__ uint32_t slots[NW][KB];
     __shared__ float mls[NW][RT][2];
     __shared__ __attribute__((aligned(16))) float os[NW][RT][OS];
     const KvTables &t = A.t;
     const KvAttend &a = A.a;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int at = blockIdx.x;
     const int h = at % t.Hk;
     at /= t.Hk;
@@ -98,111 +211,110 @@ __global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
     const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
     if (ch >= nch) return;
 
-    // this lane's query row, times scale and log2(e)
-    const int r = rt * RT + c, tok = min(r, rt * RT + tl.live - 1) / a.G;
-    const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
-    float q[NK][EL];
-    {
-        const float *qp = a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK;
-        const float f = a.scale * 1.4426950408889634f;
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            if (c < tl.live) load_run<EL>(qp + 4 * EL * i + EL * g, q[i]);
-#pragma unroll
-            for (int e = 0; e < EL; e++) q[i][e] = c < tl.live ? q[i][e] * f : 0.0f;
+    // This wave's blocks, in parts of NB tiles of 16 keys: a part's loads are all on
+    // their way before the first product (the first part's before q is looked at).
+    const int e1 = min(e0 + chunk_blocks(tl.sp.cnt), tl.sp.cnt);
+    uint32_t kr[NB][NU][4], vr[NB][4][VB / 4];
+    int j0 = 0;
+    bool all = false;   // every row sees every key of the block
+    auto fetch = [&](int e, int n0) {
+        if (n0 == 0) {
+            j0 = tl.sp.block(e) * KB;
+            const int jl = j0 + lane, jc = min(jl, tl.hi1), lp = jc / t.page;
+            const int pg = t.pages[(size_t)b * t.max_pages + lp];
+            const bool in = jl <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
+            const uint32_t at_l = in ? ((uint32_t)pg * t.Hk + h) * t.page + (jc - lp * t.page) : KV_NONE;
+            all = __builtin_amdgcn_readfirstlane(__all(in && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks)));
+            wave_lds_order();   // the reads of the last block's slots
+            slots[w][lane] = at_l;
+            wave_lds_order();
         }
-    }
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            const uint32_t at_k = slots[w][16 * (n0 + n) + c];
+            const T *kp = (const T *)t.k + (size_t)(at_k == KV_NONE ? 0 : at_k) * DK + EL * g;
+#pragma unroll
+            for (int u = 0; u < NU; u++) load_run<16>(kp + 4 * EL * u, kr[n][u]);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const uint32_t at_v = slots[w][16 * (n0 + n) + 4 * g + x];
+                load_run<VB>((const T *)t.v + (size_t)(at_v == KV_NONE ? 0 : at_v) * DK + VE * c, vr[n][x]);
+            }
+    };
+    int e = e0 + w, n0 = 0;
+    if (e < e1) fetch(e, 0);
+
+    // this lane's query row, times scale and log2(e)
+    const int r = rt * RT + min(c, tl.live - 1), tok = r / a.G;
+    const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
+    W wv;
+    wv.set_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
+             c < tl.live, g);
     float m = -INFINITY, l = 0.0f;
     f4 o[VE];
 #pragma unroll
-    for (int e = 0; e < VE; e++) o[e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = 0; x < VE; x++) o[x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int e1 = min(e0 + chunk_blocks(tl.sp.cnt), tl.sp.cnt);
-    for (int e = e0 + w; e < e1; e += NW) {
-        const int j0 = tl.sp.block(e) * KB;
-        // where the block's keys lie; `all`: every row sees every one of them
-        const int jl = j0 + lane;
-        const uint32_t at_l = jl <= tl.hi1 ? kv_slot(t, b, jl, h) : KV_NONE;
-        const bool all = __all(at_l != KV_NONE && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks));
-        wave_lds_order();   // the reads of the last block's slots
-        slots[w][lane] = at_l;
-        wave_lds_order();
-        f4 s[KB / 16];
+    while (e < e1) {
+        f4 s[NB];
 #pragma unroll
-        for (int n = 0; n < KB / 16; n++) {
-            const uint32_t at_k = slots[w][16 * n + c];
-            const T *kp = (const T *)t.k + (size_t)(at_k == KV_NONE ? 0 : at_k) * DK;
-            s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < NB; n++) s[n] = wv.scores(kr[n]);
+        // A value that only some rows see meets the others' probability 0,
+        // which hides it unless it is not finite: such an element counts as 0 in
+        // the product and is added afterwards to the rows that see it.
+        bool odd = false;
+        if (!all) {
 #pragma unroll
-            for (int i = 0; i < NK; i++) {
-                float k[EL];
-                load_run<EL>(kp + 4 * EL * i + EL * g, k);
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int x = 0; x < EL; x++) s[n] = mfma4(k[x], q[i][x], s[n]);
-            }
+                for (int x = 0; x < 4; x++) {
+                    const int jj = 16 * (n0 + n) + 4 * g + x, j = j0 + jj;
+                    const bool in = slots[w][jj] != KV_NONE;
+                    s[n][x] = in && j <= hi && (j >= lo || j < a.sinks) ? s[n][x] : -INFINITY;
+#pragma unroll
+                    for (int y = 0; y < VB / 4; y++) odd |= W::clean(vr[n][x][y]) && in;
+                }
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < KB / 16; n++)
+        for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int jj = 16 * n + 4 * g + x, j = j0 + jj;
-                if (!all) {
-                    const bool see = slots[w][jj] != KV_NONE && j <= hi && (j >= lo || j < a.sinks);
-                    s[n][x] = see ? s[n][x] : -INFINITY;
-                }
-                mx = fmaxf(mx, s[n][x]);
-            }
+            for (int x = 0; x < 4; x++) mx = fmaxf(mx, s[n][x]);
         const float mn = fmaxf(m, max_g(mx)), mz = mn == -INFINITY ? 0.0f : mn;
-        const float al = exp2f(m - mz);
+        const float al = __builtin_amdgcn_exp2f(m - mz);
         m = mn;
-        float sum = 0.0f;
+        l *= al;
 #pragma unroll
-        for (int n = 0; n < KB / 16; n++)
+        for (int n = 0; n < NB; n++)
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                s[n][x] = exp2f(s[n][x] - mz);
-                sum += s[n][x];
+                s[n][x] = __builtin_amdgcn_exp2f(s[n][x] - mz + W::TOP);
+                l += s[n][x];
             }
-        l = l * al + sum;
 #pragma unroll
         for (int x = 0; x < VE; x++) o[x] *= al;
-        // Values. A key that only some rows see meets the others' probability 0,
-        // which hides it unless it is not finite: such an element counts as 0 in
-        // the product and is added to the rows that see it afterwards.
-        bool odd = false;
-#pragma unroll
-        for (int n = 0; n < KB / 16; n++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int jj = 16 * n + 4 * g + x;
-                const uint32_t at_v = slots[w][jj];
-                float v[VE];
-                load_run<VE>((const T *)t.v + (size_t)(at_v == KV_NONE ? 0 : at_v) * DK + VE * c, v);
-                if (!all) {
-#pragma unroll
-                    for (int y = 0; y < VE; y++) {
-                        const bool fin = fabsf(v[y]) < INFINITY;
-                        odd = odd || (!fin && at_v != KV_NONE);
-                        v[y] = fin && at_v != KV_NONE ? v[y] : 0.0f;
-                    }
-                }
-#pragma unroll
-                for (int y = 0; y < VE; y++) o[y] = mfma4(v[y], s[n][x], o[y]);
-            }
+        W::context(vr, s, o);
         if (__any(odd)) {
-            for (int jj = 0; jj < KB; jj++) {
+            for (int jj = 16 * n0; jj < 16 * (n0 + NB); jj++) {
                 const uint32_t at_v = slots[w][jj];
                 const int j = j0 + jj;
                 if (at_v == KV_NONE || j > hi || (j < lo && j >= a.sinks)) continue;
                 const T *vp = (const T *)t.v + (size_t)at_v * DK;
+#pragma unroll
                 for (int x = 0; x < 4; x++)
+#pragma unroll
                     for (int y = 0; y < VE; y++) {
                         const float v = (float)vp[VE * (4 * g + x) + y];
                         if (!(fabsf(v) < INFINITY)) o[y][x] += v;
                     }
             }
         }
+        n0 += NB;
+        if (n0 == KB / 16) n0 = 0, e += NW;
+        if (e < e1) fetch(e, n0);
     }
     l = sum_g(l);
 
@@ -212,10 +324,10 @@ __global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
     float mb = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NW; i++) mb = fmaxf(mb, mls[i][c][0]);
-    const float mz = mb == -INFINITY ? 0.0f : mb, f = exp2f(m - mz);
+    const float mz = mb == -INFINITY ? 0.0f : mb, f = __builtin_amdgcn_exp2f(m - mz);
     float lb = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NW; i++) lb += mls[i][c][1] * exp2f(mls[i][c][0] - mz);
+    for (int i = 0; i < NW; i++) lb += mls[i][c][1] * __builtin_amdgcn_exp2f(mls[i][c][0] - mz);
 #pragma unroll
     for (int x = 0; x < 4; x++)
 #pragma unroll
@@ -245,7 +357,7 @@ __global__ __launch_bounds__(NTH) void k_kv_step(const StepArgs A) {
         for (int k = 0; k < NW; k++) ms = fmaxf(ms, mls[k][row][0]);
         ms = ms == -INFINITY ? 0.0f : ms;
 #pragma unroll
-        for (int k = 0; k < NW; k++) ls += mls[k][row][1] * exp2f(mls[k][row][0] - ms);
+        for (int k = 0; k < NW; k++) ls += mls[k][row][1] * __builtin_amdgcn_exp2f(mls[k][row][0] - ms);
         const int rr = rt * RT + row;
         const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
         *(f4 *)(a.out + (int64_t)(tl.s.r0 + rr / a.G) * a.ldo + (h * a.G + rr % a.G) * DK + d) = u * inv;

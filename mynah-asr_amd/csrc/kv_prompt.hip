@@ -12,16 +12,15 @@
 // 5: A row c, B column c, slots 8 hf + j; D rows 8 (e / 4) + 4 hf + e % 4, column c):
 //   S^T = K Q^T, O^T = V^T P^T
 // so a lane holds the scores of one query row, 32 of a tile's 64 keys, and its
-// probabilities are the second product's B operand as they lie. K and V are exact in
-// their type; q and the probabilities are f32, which NT terms of that type carry: f16
-// two (22 bits; q rows scaled by a power of two to the top of f16's range, probabilities
-// below 2^15), bf16 three (24 bits).
+// probabilities are the second product's B operand as they lie (their terms, and q's:
+// kv_terms.h; a q row is scaled by a power of two, probabilities stay below 2^14).
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
 // is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + 8).
 #include <hip/hip_runtime.h>
 #include <math.h>
 
 #include "kv.h"
+#include "kv_terms.h"
 #include "launch.h"
 #include "product.h"
 
@@ -30,7 +29,6 @@ namespace {
 constexpr int NW = 4, NTH = 64 * NW;
 constexpr int RT = 32 * NW;   // rows of a tile
 constexpr int KB = 64;        // keys of a tile
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -41,45 +39,6 @@ struct PromptArgs {
     KvAttend a;
     float *part;         // partial contexts [workgroup][RT][DK], then their references and sums [workgroup][RT][2]
     int ntile, nch, ct;  // tiles (at most), chunks of a tile's keys (at most), key tiles of a chunk
-};
-
-template <typename T> struct Terms;
-template <> struct Terms<_Float16> {
-    typedef half8 v8;
-    static constexpr int N = 2;
-    static __device__ __forceinline__ f16v mfma(v8 a, v8 b, f16v c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void split(const float (&x)[8], v8 (&t)[2]) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) t[0][j] = (_Float16)x[j];
-#pragma unroll
-        for (int j = 0; j < 8; j++) t[1][j] = (_Float16)fmaf(-1.0f, (float)t[0][j], x[j]);
-    }
-    // the exponent that brings a row's maximum to [2^13, 2^14)
-    static __device__ __forceinline__ int shift(float mx) {
-        int e = 0;
-        if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &e);
-        else e = 14;
-        return 14 - e;
-    }
-};
-template <> struct Terms<__bf16> {
-    typedef bf8 v8;
-    static constexpr int N = 3;
-    static __device__ __forceinline__ f16v mfma(v8 a, v8 b, f16v c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void split(const float (&x)[8], v8 (&t)[3]) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            t[0][j] = (__bf16)x[j];
-            const float r = x[j] - (float)t[0][j];
-            t[1][j] = (__bf16)r;
-            t[2][j] = (__bf16)(r - (float)t[1][j]);
-        }
-    }
-    static __device__ __forceinline__ int shift(float) { return 0; }
 };
 
 // The sequence and its row tile that tile number `at` of the call is: tiles are
@@ -117,7 +76,7 @@ __device__ __forceinline__ bool find_tile(const KvTables &t, const KvAttend &a, 
 
 template <typename T, int DK>
 __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
-    using X = Terms<T>;
+    using X = KvTerms<T>;
     typedef typename X::v8 v8;
     constexpr int NT = X::N, KS = DK / 16, DT = DK / 32;
     constexpr int CH = DK / 8;                     // 16-byte pieces of a row
@@ -217,10 +176,9 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         // product and is added afterwards to the rows that see it.
         int odd = 0;
         if (!all) {
-            constexpr uint32_t EXP = sizeof(T) == 2 && X::N == 2 ? 0x7c00u : 0x7f80u;
             for (int i = tid; i < TB / 4; i += NTH) {
                 uint32_t x = ((uint32_t *)vt)[i];
-                const bool bl = (x & EXP) == EXP, bh = (x >> 16 & EXP) == EXP;
+                const bool bl = kv_odd_lo<T>(x), bh = kv_odd_hi<T>(x);
                 if (bl || bh) {
                     odd = 1;
                     x = (bl ? 0 : x & 0xffff) | (bh ? 0 : x & 0xffff0000u);
@@ -236,7 +194,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
             for (int u = 0; u < KS; u++) {
                 const v8 k = *(const v8 *)(kt + 32 * n * (DK * 2) + kbase + ((2 * u) ^ kx) * 16);
 #pragma unroll
-                for (int x = 0; x < NT; x++) s = X::mfma(k, q[u][x], s);
+                for (int x = 0; x < NT; x++) s = X::mfma32(k, q[u][x], s);
             }
             if (!all) {
                 const uint32_t mine = (uint32_t)(okw >> (32 * n + 4 * hf));
@@ -282,7 +240,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
                     }
                     const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int x = 0; x < NT; x++) o[d] = X::mfma(vv, pt[x], o[d]);
+                    for (int x = 0; x < NT; x++) o[d] = X::mfma32(vv, pt[x], o[d]);
                 }
             }
         }
