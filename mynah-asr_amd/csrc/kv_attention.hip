@@ -81,16 +81,17 @@ template <int BYTES> __device__ __forceinline__ void load_run(const void *p, uin
 }
 
 // The two products of a wave on one kind of cache. Both take and give the f32
-// scores s[tile of 16 keys], keys 4 g + e of query row c in lane (c, g).
+// scores s[tile of 16 keys], keys 4 g + e of query row c in lane (c, g). The query
+// rows, which the workgroup's waves share, lie in LDS as fragments of 64 x 16 bytes;
+// put_q has each wave form its part of them.
 template <typename T, int DK> struct Wave {   // 16 bits
     using X = KvTerms<T>;
     typedef typename X::v8 v8;
-    static constexpr int NB = KB / 16;             // key tiles at a time
-    static constexpr int NU = DK / 32, VE = DK / 16;
+    static constexpr int NB = 2;                   // key tiles at a time
+    static constexpr int NU = DK / 32, VE = DK / 16, QF = NU * X::N;
     static constexpr float TOP = X::N == 2 ? 14.0f : 0.0f;   // probabilities reach 2^TOP
-    v8 q[NU][X::N];
     float sc;
-    __device__ __forceinline__ void set_q(const float *qp, float f, bool live, int g) {
+    __device__ __forceinline__ void put_q(const float *qp, float f, bool live, int g, int w, uint4 *ql) {
         float x[NU][8], mx = 0.0f;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
@@ -106,20 +107,29 @@ template <typename T, int DK> struct Wave {   // 16 bits
         sc = ldexpf(1.0f, -e);
 #pragma unroll
         for (int u = 0; u < NU; u++) {
+            if (u % NW != w) continue;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[u][j] = ldexpf(x[u][j], e);
-            X::split(x[u], q[u]);
+            v8 q[X::N];
+            X::split(x[u], q);
+#pragma unroll
+            for (int i = 0; i < X::N; i++) ql[64 * (X::N * u + i)] = __builtin_bit_cast(uint4, q[i]);
         }
     }
-    __device__ __forceinline__ f4 scores(const uint32_t (&k)[NU][4]) const {
-        f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void scores(const uint4 *ql, const uint32_t (&k)[NB][NU][4], f4 (&s)[NB]) const {
 #pragma unroll
-        for (int u = 0; u < NU; u++) {
-            const v8 kv = __builtin_bit_cast(v8, uint4{k[u][0], k[u][1], k[u][2], k[u][3]});
+        for (int n = 0; n < NB; n++) s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int x = 0; x < X::N; x++) s = X::mfma16(kv, q[u][x], s);
-        }
-        return s * sc;
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+            for (int i = 0; i < X::N; i++) {
+                const v8 q = __builtin_bit_cast(v8, ql[64 * (X::N * u + i)]);
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+                    s[n] = X::mfma16(__builtin_bit_cast(v8, uint4{k[n][u][0], k[n][u][1], k[n][u][2], k[n][u][3]}), q, s[n]);
+            }
+#pragma unroll
+        for (int n = 0; n < NB; n++) s[n] *= sc;
     }
     // o[e] += V^T P^T: feature VE (4 g + x) + e of the context in element x
     static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE / 2], const f4 (&p)[NB], f4 (&o)[VE]) {
@@ -151,25 +161,28 @@ template <typename T, int DK> struct Wave {   // 16 bits
     }
 };
 template <int DK> struct Wave<float, DK> {
-    static constexpr int NB = 2;                   // (twice the registers of 16 bits)
-    static constexpr int NU = DK / 16, VE = DK / 16;
+    static constexpr int NB = 1;
+    static constexpr int NU = DK / 16, VE = DK / 16, QF = NU;
     static constexpr float TOP = 0.0f;
-    float q[NU][4];
-    __device__ __forceinline__ void set_q(const float *qp, float f, bool live, int g) {
+    __device__ __forceinline__ void put_q(const float *qp, float f, bool live, int g, int w, uint4 *ql) {
 #pragma unroll
         for (int u = 0; u < NU; u++) {
+            if (u % NW != w) continue;
             const f4 x = *(const f4 *)(qp + 16 * u + 4 * g);
-#pragma unroll
-            for (int j = 0; j < 4; j++) q[u][j] = live ? x[j] * f : 0.0f;
+            ql[64 * u] = __builtin_bit_cast(uint4, live ? x * f : f4{0.0f, 0.0f, 0.0f, 0.0f});
         }
     }
-    __device__ __forceinline__ f4 scores(const uint32_t (&k)[NU][4]) const {
-        f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void scores(const uint4 *ql, const uint32_t (&k)[NB][NU][4], f4 (&s)[NB]) const {
 #pragma unroll
-        for (int u = 0; u < NU; u++)
+        for (int n = 0; n < NB; n++) s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 4; j++) s = mfma4(__uint_as_float(k[u][j]), q[u][j], s);
-        return s;
+        for (int u = 0; u < NU; u++) {
+            const f4 q = __builtin_bit_cast(f4, ql[64 * u]);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int n = 0; n < NB; n++) s[n] = mfma4(__uint_as_float(k[n][u][j]), q[j], s[n]);
+        }
     }
     static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE], const f4 (&p)[NB], f4 (&o)[VE]) {
 #pragma unroll
@@ -187,7 +200,7 @@ template <int DK> struct Wave<float, DK> {
 };
 
 template <typename T, int DK>
-__global__ __launch_bounds__(NTH, 2) void k_kv_step(const StepArgs A) {
+__global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     using W = Wave<T, DK>;
     constexpr int EL = 16 / sizeof(T);       // features of a 16-byte load
     constexpr int NB = W::NB, NU = W::NU, VE = W::VE;
@@ -195,7 +208,10 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_step(const StepArgs A) {
     constexpr int OS = DK + 4;
     __shared__ uint32_t slots[NW][KB];
     __shared__ float mls[NW][RT][2];
+    // q's fragments, then the waves' contexts
     __shared__ __attribute__((aligned(16))) float os[NW][RT][OS];
+    static_assert(W::QF * 1024 <= sizeof os, "q in LDS");
+    uint4 *ql = (uint4 *)os + (threadIdx.x & 63);
     const KvTables &t = A.t;
     const KvAttend &a = A.a;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -251,8 +267,9 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_step(const StepArgs A) {
     const int r = rt * RT + min(c, tl.live - 1), tok = r / a.G;
     const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
     W wv;
-    wv.set_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
-             c < tl.live, g);
+    wv.put_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
+             c < tl.live, g, w, ql);
+    __syncthreads();
     float m = -INFINITY, l = 0.0f;
     f4 o[VE];
 #pragma unroll
@@ -260,8 +277,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_step(const StepArgs A) {
 
     while (e < e1) {
         f4 s[NB];
-#pragma unroll
-        for (int n = 0; n < NB; n++) s[n] = wv.scores(kr[n]);
+        wv.scores(ql, kr, s);
         // A value that only some rows see meets the others' probability 0,
         // which hides it unless it is not finite: such an element counts as 0 in
         // the product and is added afterwards to the rows that see it.
@@ -387,6 +403,20 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
     const size_t wgs = (size_t)A.t.nseq * A.nrt * A.nch * A.t.Hk;
     const float *ml = A.part + wgs * A.R * DK;
     auto slot = [&](int i) { return (wg0 + (size_t)i * A.t.Hk) * A.R + row; };
+    // the first contexts are on their way while the maximum is found
+    constexpr int U = 4;
+    const int gi = tid / LN, d = 4 * (tid % LN);
+    f4 x[U];
+    float2 y[U];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const size_t s = slot(min(i0 + NG * u, nch - 1));
+            x[u] = *(const f4 *)(A.part + s * DK + d);
+            y[u] = *(const float2 *)(ml + 2 * s);
+        }
+    };
+    fetch(gi);
     float m = -INFINITY;
     for (int i = tid; i < nch; i += NTH) m = fmaxf(m, ml[2 * slot(i)]);
     m = wave_max<64>(m);
@@ -394,14 +424,17 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float mz = m == -INFINITY ? 0.0f : m;
-    const int gi = tid / LN, d = 4 * (tid % LN);
     f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
-    for (int i = gi; i < nch; i += NG) {
-        const size_t s = slot(i);
-        const float f = exp2f(ml[2 * s] - mz);
-        l += f * ml[2 * s + 1];
-        o += f * *(const f4 *)(A.part + s * DK + d);
+    for (int i0 = gi; i0 < nch; i0 += NG * U) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const bool in = i0 + NG * u < nch;
+            const float f = in ? __builtin_amdgcn_exp2f(y[u].x - mz) : 0.0f;
+            l += in ? f * y[u].y : 0.0f;
+            o += in ? f * x[u] : f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        if (i0 + NG * U < nch) fetch(i0 + NG * U);
     }
     *(f4 *)&os[gi][d] = o;
     if (d == 0) ls[gi] = l;
@@ -446,14 +479,14 @@ Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
 
 int64_t mh_kv_attention_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     if ((int64_t)a.max_new * a.G >= 1 << 30) return -1;
-    if (mh_kv_prompt(type, a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, dk, a);
+    if (mh_kv_prompt(a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, type, dk, a);
     const Plan p = plan_of(nseq, Hk, page, max_pages, a);
     if (p.wgs >= 1 << 30) return -1;
     return p.nch > 1 ? p.wgs * p.R * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
-    if (mh_kv_prompt(type, a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
+    if (mh_kv_prompt(a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
     const Plan p = plan_of(t.nseq, t.Hk, t.page, t.max_pages, a);
     const StepArgs A{t, a, ws, p.nrt, p.nch, p.R};
     auto go = [&](auto step, auto join) {

@@ -1,23 +1,27 @@
 // kv_prompt.hip — attention over a paged cache for many new rows of a sequence
-// (prompts, and parts of them) on 16-bit caches. The mathematics and the
-// visibility of keys are kv_attention.hip's.
+// (prompts, and parts of them). The mathematics and the visibility of keys are
+// kv_attention.hip's.
 //
 // One workgroup = four waves = 128 rows of one K/V head (token * G + head), 32 a
-// wave, over all the keys they see or one chunk of them; tiles of 64 keys. K and V
-// tiles go from the cache's pages to LDS as they lie (global_load_lds, two slots:
-// the next tile's copies run while this one's products do), rows swizzled so that
-// the 16-byte reads of K and the transposing reads of V meet no bank twice.
+// wave, over all the keys they see or one chunk of them; tiles of 64 keys (f32
+// caches: 32). K and V tiles go from the cache's pages to LDS as they lie
+// (global_load_lds, two slots: the next tile's copies run while this one's products
+// do), rows swizzled so that the reads below meet no bank twice.
 //
-// Products on the 32x32x16 MFMA of the cache's type (lane l, c = l & 31, hf = l >>
-// 5: A row c, B column c, slots 8 hf + j; D rows 8 (e / 4) + 4 hf + e % 4, column c):
-//   S^T = K Q^T, O^T = V^T P^T
-// so a lane holds the scores of one query row, 32 of a tile's 64 keys, and its
-// probabilities are the second product's B operand as they lie (their terms, and q's:
-// kv_terms.h; a q row is scaled by a power of two, probabilities stay below 2^14).
+// Products, S^T = K Q^T and O^T = V^T P^T (lane l, c = l & 31, hf = l >> 5: A row c,
+// B column c, D rows 8 (e / 4) + 4 hf + e % 4, column c): a lane holds the scores of
+// one query row, half of a tile's keys, and its probabilities are the second
+// product's B operand as they lie, which is free to take its keys in that order.
+//   16 bits: the 32x32x16 MFMA of the cache's type, slots 8 hf + j; value rows come
+//     transposed from LDS (ds_read_b64_tr_b16); q and probabilities in terms
+//     (kv_terms.h; a q row scaled by a power of two, probabilities below 2^14).
+//   f32: the 32x32x2 f32 MFMA, slot hf.
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
 // is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + 8).
 #include <hip/hip_runtime.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "kv.h"
 #include "kv_terms.h"
@@ -28,7 +32,7 @@ namespace {
 
 constexpr int NW = 4, NTH = 64 * NW;
 constexpr int RT = 32 * NW;   // rows of a tile
-constexpr int KB = 64;        // keys of a tile
+template <typename T> constexpr int KB = sizeof(T) == 4 ? 32 : 64;   // keys of a tile
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -40,6 +44,12 @@ struct PromptArgs {
     float *part;         // partial contexts [workgroup][RT][DK], then their references and sums [workgroup][RT][2]
     int ntile, nch, ct;  // tiles (at most), chunks of a tile's keys (at most), key tiles of a chunk
 };
+
+// the larger of the two halves' values, in both
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // The sequence and its row tile that tile number `at` of the call is: tiles are
 // numbered sequence by sequence, a sequence's last rows (in causal order the
@@ -74,16 +84,167 @@ __device__ __forceinline__ bool find_tile(const KvTables &t, const KvAttend &a, 
     return false;
 }
 
-template <typename T, int DK>
-__global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
+// A wave's operands and products on one kind of cache. at_k, at_v: where this lane's
+// first pieces of a K and a V tile lie; other rows of a tile that a lane reads differ by
+// a constant number of rows whose swizzle differs by a constant xor.
+template <typename T, int DK> struct Ops {   // 16 bits
     using X = KvTerms<T>;
     typedef typename X::v8 v8;
-    constexpr int NT = X::N, KS = DK / 16, DT = DK / 32;
-    constexpr int CH = DK / 8;                     // 16-byte pieces of a row
-    constexpr int TB = KB * DK * 2;                // bytes of a tile
+    static constexpr int KS = DK / 16, DT = DK / 32, ROW = DK * 2;
+    // K fragments of the next half are read ahead where q's terms leave the registers
+    static constexpr bool AHEAD = X::N * KS <= 16;
+    // of any 16 rows that follow each other one piece each, and of any four the four
+    // pieces that follow each other, lie in all 64 banks
+    static __device__ __forceinline__ int swz(int row) {
+        return DK == 128 ? (row & 3) * 4 + (row >> 2 & 3) : (row >> 1 & 1) * 4 + (row >> 2 & 3);
+    }
+    // feature of element x of context tile d
+    static __device__ __forceinline__ int feature(int d, int x, int hf) { return 32 * d + 8 * (x / 4) + 4 * hf + x % 4; }
+    v8 q[KS][X::N];
+    float sc;   // what turns a sum of products into a score, in powers of two
+    int at_k, at_v;
+    __device__ __forceinline__ void init(const float *qp, float f, bool live, int lane) {
+        const int c = lane & 31, hf = lane >> 5, vrow = 4 * hf + (lane & 15) / 4;
+        at_k = c * ROW + (hf ^ swz(c)) * 16;
+        at_v = vrow * ROW + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz(vrow)) * 16 + 8 * (lane & 1);
+        float x[KS][8], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            *(f4 *)&x[s][0] = *(const f4 *)(qp + 16 * s + 8 * hf);
+            *(f4 *)&x[s][4] = *(const f4 *)(qp + 16 * s + 8 * hf + 4);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[s][j] = live ? x[s][j] * f : 0.0f;
+                mx = fmaxf(mx, fabsf(x[s][j]));
+            }
+        }
+        const int e = X::shift(max_halves(mx));
+        sc = ldexpf(1.0f, -e);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
+            X::split(x[s], q[s]);
+        }
+    }
+    // The products of a tile around `soft`, which turns half n's scores into
+    // probabilities. kt, vt: the tile; ka, va: at_k, at_v.
+    template <typename F>
+    __device__ __forceinline__ void tile(const uint8_t *kt, const uint8_t *vt, int ka, int va, f16v (&o)[DT], F soft) const {
+        auto k_frag = [&](int n, int u) { return *(const v8 *)(kt + 32 * n * ROW + (ka ^ 32 * u)); };
+        auto v_frag = [&](int n, int g, int d) {   // slots 8 hf + j: keys 32 n + 16 g + 4 hf + j, from j = 4 on 8 further
+            s4 v[2];
+#pragma unroll
+            for (int y = 0; y < 2; y++)
+                v[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4 *)(vt + (32 * n + 16 * g + 8 * y) * ROW + (va ^ (64 * d + 32 * y))));
+            return __builtin_bit_cast(v8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        v8 kf[KS], vf[2][DT];
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int u = 0; u < KS; u++) kf[u] = k_frag(0, u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            f16v s = zero16();
+#pragma unroll
+            for (int u = 0; u < KS; u++) {
+                if constexpr (!AHEAD) kf[u] = k_frag(n, u);
+#pragma unroll
+                for (int x = 0; x < X::N; x++) s = X::mfma32(kf[u], q[u][x], s);
+            }
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int g = 0; g < 2; g++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) vf[g][d] = v_frag(n, g, d);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            soft(n, s, sc);
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                float p[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) p[x] = s[8 * g + x];
+                v8 pt[X::N];
+                X::split(p, pt);
+                if constexpr (AHEAD)
+                    if (g == 0 && n == 0) {
+#pragma unroll
+                        for (int u = 0; u < KS; u++) kf[u] = k_frag(1, u);
+                    }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    if constexpr (!AHEAD) vf[g][d] = v_frag(n, g, d);
+#pragma unroll
+                    for (int x = 0; x < X::N; x++) o[d] = X::mfma32(vf[g][d], pt[x], o[d]);
+                }
+            }
+        }
+    }
+    // two packed elements: those that are not finite set to 0; whether there are any
+    static __device__ __forceinline__ bool clean(uint32_t &x) {
+        const bool l = kv_odd_lo<T>(x), h = kv_odd_hi<T>(x);
+        x = (l ? 0u : x & 0xffffu) | (h ? 0u : x & 0xffff0000u);
+        return l || h;
+    }
+};
+template <int DK> struct Ops<float, DK> {
+    static constexpr int KS = DK / 8, DT = DK / 32, ROW = DK * 4;
+    static __device__ __forceinline__ int swz(int row) { return row & 15; }   // (of any 16 rows one piece each, in all banks)
+    static __device__ __forceinline__ int feature(int d, int x, int hf) { return DT * (8 * (x / 4) + 4 * hf + x % 4) + d; }
+    float q[KS][4];
+    int at_k, at_v;
+    __device__ __forceinline__ void init(const float *qp, float f, bool live, int lane) {
+        const int c = lane & 31, hf = lane >> 5;
+        at_k = c * ROW + (hf ^ swz(c)) * 16;
+        at_v = 4 * hf * ROW + ((DT * c / 4) ^ swz(4 * hf)) * 16 + DT * c % 4 * 4;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const f4 x = *(const f4 *)(qp + 8 * s + 4 * hf);
+#pragma unroll
+            for (int j = 0; j < 4; j++) q[s][j] = live ? x[j] * f : 0.0f;
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void tile(const uint8_t *kt, const uint8_t *vt, int ka, int va, f16v (&o)[DT], F soft) const {
+        f16v s = zero16();
+#pragma unroll
+        for (int u = 0; u < KS; u++) {
+            const f4 k = *(const f4 *)(kt + (ka ^ 32 * u));
+#pragma unroll
+            for (int j = 0; j < 4; j++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[u][j], s, 0, 0, 0);
+        }
+        soft(0, s, 1.0f);
+#pragma unroll
+        for (int x = 0; x < 16; x++) {   // slot hf: key 8 (x / 4) + 4 hf + x % 4, features DT c ..
+            typedef float fd __attribute__((ext_vector_type(DT)));
+            const fd v = *(const fd *)(vt + (8 * (x / 4) + x % 4) * ROW + (va ^ (8 * (x / 4 & 1) + x % 4) * 16));
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d], s[x], o[d], 0, 0, 0);
+        }
+    }
+    static __device__ __forceinline__ bool clean(uint32_t &x) {
+        const bool odd = !(fabsf(__uint_as_float(x)) < INFINITY);
+        x = odd ? 0u : x;
+        return odd;
+    }
+};
+
+template <typename T, int DK>
+__global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
+    using W = Ops<T, DK>;
+    constexpr int DT = W::DT, KT = KB<T>;
+    constexpr int CH = W::ROW / 16;                // 16-byte pieces of a row
+    constexpr int TB = KT * W::ROW;                // bytes of a tile
+    constexpr int WR = KT / NW;                    // rows of a tile that a wave copies
     constexpr int RPI = 64 / CH;                   // rows of one copy instruction
     __shared__ __attribute__((aligned(16))) uint8_t k0[TB], k1[TB], v0[TB], v1[TB];
-    __shared__ __attribute__((aligned(8))) uint16_t valid[2][NW];
+    typedef typename std::conditional<KT == 64, uint16_t, uint8_t>::type Bits;   // one a row that a wave copies
+    typedef typename std::conditional<KT == 64, uint64_t, uint32_t>::type Word;
+    __shared__ __attribute__((aligned(8))) Bits valid[2][NW];
     const KvTables &t = A.t;
     const KvAttend &a = A.a;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
@@ -95,82 +256,55 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     if (!find_tile(t, a, at % A.ntile, b, rt)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     rt = __builtin_amdgcn_readfirstlane(rt);
-    const KvTile tl = kv_tile<RT, KB>(t, a, b, rt);
+    const KvTile tl = kv_tile<RT, KT>(t, a, b, rt);
     const int ch = at / A.ntile, nch = max((tl.sp.cnt + A.ct - 1) / A.ct, 1);
     if (ch >= nch) return;
     const int e0 = ch * A.ct, e1 = min(e0 + A.ct, tl.sp.cnt);
 
-    // this lane's row: its keys, and q in terms
+    // this lane's row and its keys
     const int r = 32 * w + c, tok = (rt * RT + min(r, tl.live - 1)) / a.G;
     const int head = h * a.G + (rt * RT + min(r, tl.live - 1)) % a.G;
     const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
-    v8 q[KS][NT];
-    float sc;   // what turns a sum of products into a score, in powers of two
-    {
-        const float *qp = a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + head * DK + 8 * hf;
-        const float f = r < tl.live ? a.scale * 1.4426950408889634f : 0.0f;
-        float x[KS][8], mx = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            *(f4 *)&x[s][0] = *(const f4 *)(qp + 16 * s);
-            *(f4 *)&x[s][4] = *(const f4 *)(qp + 16 * s + 4);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[s][j] = r < tl.live ? x[s][j] * f : 0.0f;
-                mx = fmaxf(mx, fabsf(x[s][j]));
-            }
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const int e = X::shift(mx);
-        sc = ldexpf(1.0f, -e);
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
-            X::split(x[s], q[s]);
-        }
-    }
+    W wv;
+    wv.init(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + head * DK, a.scale * 1.4426950408889634f, r < tl.live, lane);
     f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = zero16();
     float m = -INFINITY, l = 0.0f;
 
-    // A piece of a row lies at its own place with the row's low bits exchanged into it.
-    auto swz = [](int row) { return DK == 128 ? row & 15 : (row >> 1) & 7; };
-    // Wave w copies rows 16 w .. of a tile; its lanes 0 .. 15 (and again 16 .. ) hold
-    // their pages, read from the table a tile ahead and looked at when they are used.
-    const int lrow = 16 * w + (lane & 15);
+    // Wave w copies rows WR w .. of a tile; its lanes 0 .. WR - 1 (and again from WR on)
+    // hold their pages, read from the table a tile ahead and looked at when they are used.
+    const int lrow = WR * w + lane % WR;
     auto page_of = [&](int e) {
-        const int j = min(tl.sp.block(min(e, e1 - 1)) * KB + lrow, tl.hi1);
+        const int j = min(tl.sp.block(min(e, e1 - 1)) * KT + lrow, tl.hi1);
         return t.pages[(size_t)b * t.max_pages + j / t.page];
     };
-    auto copy = [&](int e, int pg, uint8_t *kd, uint8_t *vd, uint16_t *ok) {
-        const int j = tl.sp.block(e) * KB + lrow;
+    auto copy = [&](int e, int pg, uint8_t *kd, uint8_t *vd, Bits *ok) {
+        const int j = tl.sp.block(e) * KT + lrow;
         const bool have = j <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
         const uint32_t sl = have ? ((uint32_t)pg * t.Hk + h) * t.page + j % t.page : 0;
-        const uint64_t ball = __ballot(have) & 0xffff;
-        if (lane == 0) ok[w] = (uint16_t)ball;
+        const uint64_t ball = __ballot(have) & ((1u << WR) - 1);
+        if (lane == 0) ok[w] = (Bits)ball;
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; i++) {
+        for (int i = 0; i < WR / RPI; i++) {
             const int rr = RPI * i + lane / CH;
-            const size_t off = (size_t)(uint32_t)__shfl((int)sl, rr, 64) * (DK * 2) + (((lane % CH) ^ swz(rr)) * 16);
+            const size_t off = (size_t)(uint32_t)__shfl((int)sl, rr, 64) * W::ROW + (((lane % CH) ^ W::swz(WR * w + rr)) * 16);
             __builtin_amdgcn_global_load_lds((const glob_void *)((const uint8_t *)t.k + off),
-                                             (lds_void *)(kd + (16 * w + RPI * i) * (DK * 2)), 16, 0, 0);
+                                             (lds_void *)(kd + (WR * w + RPI * i) * W::ROW), 16, 0, 0);
             __builtin_amdgcn_global_load_lds((const glob_void *)((const uint8_t *)t.v + off),
-                                             (lds_void *)(vd + (16 * w + RPI * i) * (DK * 2)), 16, 0, 0);
+                                             (lds_void *)(vd + (WR * w + RPI * i) * W::ROW), 16, 0, 0);
         }
     };
-    auto tile = [&](int e, const uint8_t *kt, uint8_t *vt, const uint16_t *ok) {
-        // this lane's pieces of a tile (formed anew for each: kept, they would cost registers
-        // that the products need)
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const int kbase = (ln & 31) * (DK * 2), kx = (ln >> 5) ^ swz(ln & 31);
-        const int vkey = 4 * (ln >> 5) + (ln & 15) / 4, vp = 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1);
-        const int j0 = tl.sp.block(e) * KB;
-        const uint64_t okw = *(const uint64_t *)ok;
-        const bool all = __builtin_amdgcn_readfirstlane(okw == ~0ull && j0 + KB - 1 <= tl.hi0 &&
-                                                        (j0 >= tl.lo1 || j0 + KB <= a.sinks));
+
+    auto tile = [&](int e, const uint8_t *kt, uint8_t *vt, const Bits *ok) {
+        // (opaque: the addresses formed from these, kept for every tile, would cost
+        // registers that the products need)
+        int ka = wv.at_k, va = wv.at_v;
+        asm volatile("" : "+v"(ka), "+v"(va));
+        const int j0 = tl.sp.block(e) * KT;
+        const Word okw = *(const Word *)ok;
+        const bool all = __builtin_amdgcn_readfirstlane(okw == (Word)~0ull && j0 + KT - 1 <= tl.hi0 &&
+                                                        (j0 >= tl.lo1 || j0 + KT <= a.sinks));
         // A value that only some rows see meets the others' probability 0, which
         // hides it unless it is not finite: such an element counts as 0 in the
         // product and is added afterwards to the rows that see it.
@@ -178,24 +312,14 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         if (!all) {
             for (int i = tid; i < TB / 4; i += NTH) {
                 uint32_t x = ((uint32_t *)vt)[i];
-                const bool bl = kv_odd_lo<T>(x), bh = kv_odd_hi<T>(x);
-                if (bl || bh) {
+                if (W::clean(x)) {
                     odd = 1;
-                    x = (bl ? 0 : x & 0xffff) | (bh ? 0 : x & 0xffff0000u);
                     ((uint32_t *)vt)[i] = x;
                 }
             }
             odd = __syncthreads_or(odd);
         }
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-            f16v s = zero16();
-#pragma unroll
-            for (int u = 0; u < KS; u++) {
-                const v8 k = *(const v8 *)(kt + 32 * n * (DK * 2) + kbase + ((2 * u) ^ kx) * 16);
-#pragma unroll
-                for (int x = 0; x < NT; x++) s = X::mfma32(k, q[u][x], s);
-            }
+        wv.tile(kt, vt, ka, va, o, [&](int n, f16v &s, float sc) {
             if (!all) {
                 const uint32_t mine = (uint32_t)(okw >> (32 * n + 4 * hf));
 #pragma unroll
@@ -208,7 +332,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
             float mx = s[0];
 #pragma unroll
             for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
+            mx = max_halves(mx) * sc;
             const bool up = mx > m + 6.0f;   // (m = -inf: any finite maximum)
             if (__any(up)) {
                 const float al = up ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
@@ -219,33 +343,13 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
             }
             const float sub = 8.0f - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                float p[8];
-#pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    p[x] = __builtin_amdgcn_exp2f(fmaf(s[8 * g + x], sc, sub));
-                    l += p[x];
-                }
-                v8 pt[NT];
-                X::split(p, pt);
-                // slots 8 hf + x: keys 32 n + 16 g + 4 hf + x (x < 4) and 8 further on
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    s4 v[2];
-#pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        const int key = 32 * n + 16 * g + 8 * y + vkey;
-                        v[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s4 *)(vt + key * (DK * 2) + ((4 * d + vp) ^ swz(key)) * 16 + 8 * (ln & 1)));
-                    }
-                    const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int x = 0; x < NT; x++) o[d] = X::mfma32(vv, pt[x], o[d]);
-                }
+            for (int x = 0; x < 16; x++) {
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sc, sub));
+                l += s[x];
             }
-        }
+        });
         if (odd) {
-            for (int jj = 0; jj < KB; jj++) {
+            for (int jj = 0; jj < KT; jj++) {
                 const int j = j0 + jj;
                 if (!(okw >> jj & 1) || j > hi || (j < lo && j >= a.sinks)) continue;
                 const T *vr = (const T *)t.v + (size_t)kv_slot(t, b, j, h) * DK;
@@ -253,7 +357,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
-                        const float v = (float)vr[32 * d + 8 * (x / 4) + 4 * hf + x % 4];
+                        const float v = (float)vr[W::feature(d, x, hf)];
                         if (!(fabsf(v) < INFINITY)) o[d][x] += v;
                     }
             }
@@ -280,31 +384,32 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     }
     l += __shfl_xor(l, 32, 64);
     if (r >= tl.live) return;
-    if (nch == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        float *op = a.out + (int64_t)(tl.s.r0 + tok) * a.ldo + head * DK + 4 * hf;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int x = 0; x < 16; x += 4)
-                *(f4 *)(op + 32 * d + 2 * x) = f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]} * inv;
-        return;
-    }
     const size_t slot = (size_t)blockIdx.x * RT + r;
-    float *op = A.part + slot * DK + 4 * hf;
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int x = 0; x < 16; x += 4) *(f4 *)(op + 32 * d + 2 * x) = f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
-    if (hf == 0) {
+    const float f = nch > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float *op = nch > 1 ? A.part + slot * DK : a.out + (int64_t)(tl.s.r0 + tok) * a.ldo + head * DK;
+    if (nch > 1 && hf == 0) {
         float *ml = A.part + (size_t)gridDim.x * RT * DK + 2 * slot;
         ml[0] = m;
         ml[1] = l;
     }
+    // runs of four features: of one context tile's elements (16 bits), or across the tiles
+    if constexpr (sizeof(T) == 2 || DT == 2) {
+#pragma unroll
+        for (int d = 0; d < (sizeof(T) == 2 ? DT : 1); d++)
+#pragma unroll
+            for (int x = 0; x < 16; x += sizeof(T) == 2 ? 4 : 2) {
+                const f4 u = sizeof(T) == 2 ? f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}
+                                            : f4{o[0][x], o[DT / 2][x], o[0][x + 1], o[DT / 2][x + 1]};
+                *(f4 *)(op + W::feature(d, x, hf)) = u * f;
+            }
+    } else {
+#pragma unroll
+        for (int x = 0; x < 16; x++) *(f4 *)(op + W::feature(0, x, hf)) = f4{o[0][x], o[1][x], o[2][x], o[3][x]} * f;
+    }
 }
 
 // The chunks of a tile's rows, joined in their order, as k_kv_join.
-template <int DK>
+template <typename T, int DK>
 __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
     constexpr int LN = DK / 4, RB = NTH / LN;   // lanes of a row, rows of a workgroup
     int at = blockIdx.x;
@@ -312,7 +417,7 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
     at /= A.t.Hk;
     int b, rt;
     if (!find_tile(A.t, A.a, at, b, rt)) return;
-    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
+    const KvTile tl = kv_tile<RT, KB<T>>(A.t, A.a, b, rt);
     const int nch = (tl.sp.cnt + A.ct - 1) / A.ct, row = blockIdx.y * RB + threadIdx.x / LN;
     if (nch <= 1 || row >= tl.live) return;
     const int d = 4 * (threadIdx.x % LN);
@@ -342,18 +447,18 @@ struct Plan {
     int ntile, nch, ct;
     int64_t wgs;
 };
-Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, const KvAttend &a) {
+Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const KvAttend &a) {
     Plan p;
     const int64_t per = ((int64_t)a.max_new * a.G + RT - 1) / RT;
     const int64_t most = ((int64_t)rows * a.G + RT - 1) / RT + nseq;
     const int64_t ntile = nseq * per < most ? nseq * per : most;
     const int64_t cap = (int64_t)max_pages * page;
     const int64_t keys = a.max_len < cap ? a.max_len : cap;
-    int64_t blocks = (keys + KB - 1) / KB;
+    int64_t blocks = (keys + kb - 1) / kb;
     if (a.window) {
         // a tile's rows are up to ceil(RT / G) tokens apart; each end of each part may cut a block
         const int64_t toks = (RT + a.G - 1) / a.G + 1;
-        const int64_t win = ((int64_t)a.window + toks + KB - 1) / KB + 1, sink = ((int64_t)a.sinks + KB - 1) / KB + 1;
+        const int64_t win = ((int64_t)a.window + toks + kb - 1) / kb + 1, sink = ((int64_t)a.sinks + kb - 1) / kb + 1;
         if (win + sink < blocks) blocks = win + sink;
     }
     if (blocks < 1) blocks = 1;
@@ -371,16 +476,16 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, const KvAttend
 }  // namespace
 
 // Measured crossing of the two forms: see mh_launch_kv_attention.
-bool mh_kv_prompt(int type, const KvAttend &a) { return type != KV_F32 && (int64_t)a.max_new * a.G > 64; }
+bool mh_kv_prompt(const KvAttend &a) { return (int64_t)a.max_new * a.G > 64; }
 
-int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int dk, const KvAttend &a) {
-    const Plan p = plan_of(nseq, rows, Hk, page, max_pages, a);
+int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
+    const Plan p = plan_of(nseq, rows, Hk, page, max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
     if (p.wgs >= 1 << 30) return -1;
     return p.nch > 1 ? p.wgs * RT * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_prompt(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
-    const Plan p = plan_of(t.nseq, t.rows, t.Hk, t.page, t.max_pages, a);
+    const Plan p = plan_of(t.nseq, t.rows, t.Hk, t.page, t.max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
     const PromptArgs A{t, a, ws, p.ntile, p.nch, p.ct};
     auto go = [&](auto step, auto join) {
         hipLaunchKernelGGL(step, dim3((unsigned)p.wgs), dim3(NTH), 0, st, A);
@@ -390,8 +495,10 @@ hipError_t mh_launch_kv_prompt(const KvTables &t, int type, int dk, const KvAtte
         return hipGetLastError();
     };
     if (dk == 128)
-        return type == KV_F16 ? go(k_kv_prompt<_Float16, 128>, k_kv_prompt_join<128>)
-                              : go(k_kv_prompt<__bf16, 128>, k_kv_prompt_join<128>);
-    return type == KV_F16 ? go(k_kv_prompt<_Float16, 64>, k_kv_prompt_join<64>)
-                          : go(k_kv_prompt<__bf16, 64>, k_kv_prompt_join<64>);
+        return type == KV_F32 ? go(k_kv_prompt<float, 128>, k_kv_prompt_join<float, 128>)
+               : type == KV_F16 ? go(k_kv_prompt<_Float16, 128>, k_kv_prompt_join<_Float16, 128>)
+                                : go(k_kv_prompt<__bf16, 128>, k_kv_prompt_join<__bf16, 128>);
+    return type == KV_F32 ? go(k_kv_prompt<float, 64>, k_kv_prompt_join<float, 64>)
+           : type == KV_F16 ? go(k_kv_prompt<_Float16, 64>, k_kv_prompt_join<_Float16, 64>)
+                            : go(k_kv_prompt<__bf16, 64>, k_kv_prompt_join<__bf16, 64>);
 }

@@ -6,7 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 
-#include "fmt.h"
+#include "product.h"
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
@@ -22,10 +22,14 @@ template <> struct KvTerms<_Float16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
     static __device__ __forceinline__ void split(const float (&x)[8], v8 (&t)[2]) {
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) t[0][j] = (_Float16)x[j];
-#pragma unroll
-        for (int j = 0; j < 8; j++) t[1][j] = (_Float16)fmaf(-1.0f, (float)t[0][j], x[j]);
+        for (int j = 0; j < 4; j++) {
+            h[j] = __builtin_bit_cast(uint32_t, half2v{(_Float16)x[2 * j], (_Float16)x[2 * j + 1]});
+            l[j] = lo_pair(h[j], x[2 * j], x[2 * j + 1]);
+        }
+        t[0] = __builtin_bit_cast(v8, uint4{h[0], h[1], h[2], h[3]});
+        t[1] = __builtin_bit_cast(v8, uint4{l[0], l[1], l[2], l[3]});
     }
     // the exponent that brings a row's maximum to [2^13, 2^14), near the top of f16's
     // range: the second term of what matters is then no subnormal
@@ -45,14 +49,24 @@ template <> struct KvTerms<__bf16> {
     static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    // x0, x1 rounded to a pair of bf16, and what that leaves of them
+    static __device__ __forceinline__ uint32_t pair(float &x0, float &x1) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const uint32_t h = __builtin_bit_cast(uint32_t, b2{(__bf16)x0, (__bf16)x1});
+        x0 -= __uint_as_float(h << 16);
+        x1 -= __uint_as_float(h & 0xffff0000u);
+        return h;
+    }
     static __device__ __forceinline__ void split(const float (&x)[8], v8 (&t)[3]) {
+        uint32_t h[3][4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            t[0][j] = (__bf16)x[j];
-            const float r = x[j] - (float)t[0][j];
-            t[1][j] = (__bf16)r;
-            t[2][j] = (__bf16)(r - (float)t[1][j]);
+        for (int j = 0; j < 4; j++) {
+            float x0 = x[2 * j], x1 = x[2 * j + 1];
+#pragma unroll
+            for (int k = 0; k < 3; k++) h[k][j] = pair(x0, x1);
         }
+#pragma unroll
+        for (int k = 0; k < 3; k++) t[k] = __builtin_bit_cast(v8, uint4{h[k][0], h[k][1], h[k][2], h[k][3]});
     }
     static __device__ __forceinline__ int shift(float) { return 0; }
 };
