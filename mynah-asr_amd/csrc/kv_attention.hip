@@ -199,6 +199,8 @@ template <int DK> struct Wave<float, DK> {
     }
 };
 
+__device__ __attribute__((aligned(16))) const float kv_zeros[128] = {};
+
 template <typename T, int DK>
 __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     using W = Wave<T, DK>;
@@ -230,21 +232,24 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     // This wave's blocks, in parts of NB tiles of 16 keys: a part's loads are all on
     // their way before the first product (the first part's before q is looked at).
     const int e1 = min(e0 + chunk_blocks(tl.sp.cnt), tl.sp.cnt);
+    const bool alike = tl.lo0 == tl.lo1 && tl.hi0 == tl.hi1;   // every row sees the same keys
     uint32_t kr[NB][NU][4], vr[NB][4][VB / 4];
     int j0 = 0;
-    bool all = false;   // every row sees every key of the block
-    auto fetch = [&](int e, int n0) {
-        if (n0 == 0) {
-            j0 = tl.sp.block(e) * KB;
-            const int jl = j0 + lane, jc = min(jl, tl.hi1), lp = jc / t.page;
-            const int pg = t.pages[(size_t)b * t.max_pages + lp];
-            const bool in = jl <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
-            const uint32_t at_l = in ? ((uint32_t)pg * t.Hk + h) * t.page + (jc - lp * t.page) : KV_NONE;
-            all = __builtin_amdgcn_readfirstlane(__all(in && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks)));
-            wave_lds_order();   // the reads of the last block's slots
-            slots[w][lane] = at_l;
-            wave_lds_order();
-        }
+    uint64_t some = 0, all = 0;   // of the block's keys, those that some row sees, and every row
+    auto look = [&](int e) {      // where the block's keys lie
+        j0 = tl.sp.block(e) * KB;
+        const int jl = j0 + lane, jc = min(jl, tl.hi1), lp = jc / t.page;
+        const int pg = t.pages[(size_t)b * t.max_pages + lp];
+        const bool in = jl <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
+        const bool seen = in && (jl >= tl.lo0 || jl < a.sinks);
+        some = __ballot(seen);
+        all = __ballot(in && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks));
+        wave_lds_order();   // the reads of the last block's slots
+        slots[w][lane] = seen ? ((uint32_t)pg * t.Hk + h) * t.page + (jc - lp * t.page) : KV_NONE;
+        wave_lds_order();
+    };
+    auto part = [&](uint64_t m, int n0) { return (uint32_t)(m >> (16 * n0)) & (uint32_t)((1ull << (16 * NB)) - 1); };
+    auto fetch = [&](int n0) {
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             const uint32_t at_k = slots[w][16 * (n0 + n) + c];
@@ -257,11 +262,26 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const uint32_t at_v = slots[w][16 * (n0 + n) + 4 * g + x];
-                load_run<VB>((const T *)t.v + (size_t)(at_v == KV_NONE ? 0 : at_v) * DK + VE * c, vr[n][x]);
+                // (a key that no row sees: its probability 0 times 0)
+                const T *vp = at_v == KV_NONE ? (const T *)kv_zeros : (const T *)t.v + (size_t)at_v * DK;
+                load_run<VB>(vp + VE * c, vr[n][x]);
             }
     };
+    // the next part that a row sees keys of, from (e, n0) on; false: there is none
+    auto seek = [&](int &e, int &n0) {
+        for (;;) {
+            if (n0 == 0) {
+                if (e >= e1) return false;
+                look(e);
+            }
+            if (part(some, n0)) return true;
+            n0 += NB;
+            if (n0 == KB / 16) n0 = 0, e += NW;
+        }
+    };
     int e = e0 + w, n0 = 0;
-    if (e < e1) fetch(e, 0);
+    bool more = seek(e, n0);
+    if (more) fetch(n0);
 
     // this lane's query row, times scale and log2(e)
     const int r = rt * RT + min(c, tl.live - 1), tok = r / a.G;
@@ -275,24 +295,30 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
 #pragma unroll
     for (int x = 0; x < VE; x++) o[x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    while (e < e1) {
+    while (more) {
         f4 s[NB];
         wv.scores(ql, kr, s);
-        // A value that only some rows see meets the others' probability 0,
-        // which hides it unless it is not finite: such an element counts as 0 in
-        // the product and is added afterwards to the rows that see it.
         bool odd = false;
-        if (!all) {
+        if (part(all, n0) != part(~0ull, 0)) {
+            const uint32_t see = part(some, n0) >> (4 * g);
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const int jj = 16 * (n0 + n) + 4 * g + x, j = j0 + jj;
-                    const bool in = slots[w][jj] != KV_NONE;
-                    s[n][x] = in && j <= hi && (j >= lo || j < a.sinks) ? s[n][x] : -INFINITY;
-#pragma unroll
-                    for (int y = 0; y < VB / 4; y++) odd |= W::clean(vr[n][x][y]) && in;
+                    const int j = j0 + 16 * (n0 + n) + 4 * g + x;
+                    s[n][x] = (see >> (16 * n + x) & 1) && j <= hi && (j >= lo || j < a.sinks) ? s[n][x] : -INFINITY;
                 }
+            // A value that only some rows see meets the others' probability 0, which
+            // hides it unless it is not finite: such an element counts as 0 in the
+            // product and is added afterwards to the rows that see it.
+            if (!alike) {
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int y = 0; y < VB / 4; y++) odd |= W::clean(vr[n][x][y]);
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -330,7 +356,8 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
         }
         n0 += NB;
         if (n0 == KB / 16) n0 = 0, e += NW;
-        if (e < e1) fetch(e, n0);
+        more = seek(e, n0);
+        if (more) fetch(n0);
     }
     l = sum_g(l);
 
