@@ -55,27 +55,38 @@ __global__ __launch_bounds__(NTH) void k_kv_append(const KvTables t, const KvApp
     constexpr int UN = NTH / TP;        // heads at a time
     __shared__ float2 cs[DK / 2];
     const int row = blockIdx.x, tid = threadIdx.x, l = tid % TP;
+    const bool split = !a.inter && l < a.rot / 8;
+    const int e0 = split ? 4 * l : 8 * l, e1 = split ? a.rot / 2 + 4 * l : 8 * l + 4;
+    const int units = a.Hq + 2 * t.Hk;
+    // what the row's sequence has no part in is on its way before that is known
+    f4 x0, x1;
+    auto load = [&](int u) {
+        const float *x = u < a.Hq ? a.q + row * a.ldq + u * DK
+                         : u < a.Hq + t.Hk ? a.k + row * a.ldk + (u - a.Hq) * DK
+                                           : a.v + row * a.ldv + (u - a.Hq - t.Hk) * DK;
+        x0 = *(const f4 *)(x + e0);
+        x1 = *(const f4 *)(x + e1);
+    };
+    int u = blockIdx.y * UN + tid / TP;
+    if (u < units) load(u);
+    const double freq = tid < a.rot / 2 ? a.freq[tid] * 0.15915494309189533577 : 0.0;   // turns: 1 / (2 pi)
     const int b = find_seq(t.row_start, t.nseq, row);
     if (b >= t.nseq) return;            // behind the last sequence
     const KvSeq s = kv_seq(t, b);
     if (row < s.r0 || row - s.r0 >= s.n) return;   // (before the first)
     const int p = s.L - s.n + (row - s.r0);
+    const bool in_pool = p >= 0 && p / t.page < t.max_pages;
+    const uint32_t at0 = in_pool ? kv_slot(t, b, p, 0) : KV_NONE;   // of head 0; a head's slots follow the one before's
     if (tid < a.rot / 2) {
-        const double turns = (double)p * a.freq[tid] * 0.15915494309189533577;   // 1 / (2 pi)
+        const double turns = (double)p * freq;
         float sn, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &sn, &c);
         cs[tid] = make_float2(c, sn);
     }
     __syncthreads();
-    const bool split = !a.inter && l < a.rot / 8;
-    const int e0 = split ? 4 * l : 8 * l, e1 = split ? a.rot / 2 + 4 * l : 8 * l + 4;
-    const bool in_pool = p >= 0 && p / t.page < t.max_pages;
-    const int units = a.Hq + 2 * t.Hk;
-    for (int u = blockIdx.y * UN + tid / TP; u < units; u += gridDim.y * UN) {
+    for (; u < units; u += gridDim.y * UN) {
         const bool isq = u < a.Hq, isv = u >= a.Hq + t.Hk;
         const int h = isq ? u : isv ? u - a.Hq - t.Hk : u - a.Hq;
-        const float *x = (isq ? a.q + row * a.ldq : isv ? a.v + row * a.ldv : a.k + row * a.ldk) + h * DK;
-        f4 x0 = *(const f4 *)(x + e0), x1 = *(const f4 *)(x + e1);
         const float *w = isv ? nullptr : isq ? a.qn : a.kn;
         if (w) {
             double ss = 0.0;
@@ -109,14 +120,12 @@ __global__ __launch_bounds__(NTH) void k_kv_append(const KvTables t, const KvApp
             float *o = a.qo + row * a.ldqo + h * DK;
             *(f4 *)(o + e0) = x0;
             *(f4 *)(o + e1) = x1;
-        } else if (in_pool) {
-            const uint32_t at = kv_slot(t, b, p, h);
-            if (at != KV_NONE) {
-                T *o = (T *)(isv ? t.v : t.k) + (size_t)at * DK;
-                store4(o + e0, x0);
-                store4(o + e1, x1);
-            }
+        } else if (at0 != KV_NONE) {
+            T *o = (T *)(isv ? t.v : t.k) + ((size_t)at0 + (size_t)h * t.page) * DK;
+            store4(o + e0, x0);
+            store4(o + e1, x1);
         }
+        if (u + (int)gridDim.y * UN < units) load(u + gridDim.y * UN);
     }
 }
 

@@ -221,9 +221,9 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     int at = blockIdx.x;
     const int h = at % t.Hk;
     at /= t.Hk;
-    const int ch = at % A.nch;
-    at /= A.nch;
-    const int rt = at % A.nrt, b = at / A.nrt;
+    const int rt = at % A.nrt;   // (the tiles that read the same keys run together, on one XCD where Hk is a multiple of 8)
+    at /= A.nrt;
+    const int ch = at % A.nch, b = at / A.nch;
     const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
     if (tl.live <= 0) return;
     const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
@@ -425,11 +425,11 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
     if (row >= tl.live) return;
     const int nch = chunks_of(tl.sp.cnt);
     if (nch <= 1) return;
-    // chunk i's workgroup: ((b nrt + rt) nch_max + i) Hk + h
-    const size_t wg0 = ((size_t)b * A.nrt + rt) * A.nch * A.t.Hk + h;
+    // chunk i's workgroup: ((b nch_max + i) nrt + rt) Hk + h
+    const size_t wg0 = ((size_t)b * A.nch * A.nrt + rt) * A.t.Hk + h;
     const size_t wgs = (size_t)A.t.nseq * A.nrt * A.nch * A.t.Hk;
     const float *ml = A.part + wgs * A.R * DK;
-    auto slot = [&](int i) { return (wg0 + (size_t)i * A.t.Hk) * A.R + row; };
+    auto slot = [&](int i) { return (wg0 + (size_t)i * A.nrt * A.t.Hk) * A.R + row; };
     // the first contexts are on their way while the maximum is found
     constexpr int U = 4;
     const int gi = tid / LN, d = 4 * (tid % LN);
@@ -506,14 +506,14 @@ Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
 
 int64_t mh_kv_attention_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     if ((int64_t)a.max_new * a.G >= 1 << 30) return -1;
-    if (mh_kv_prompt(a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, type, dk, a);
+    if (mh_kv_prompt(type, a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, type, dk, a);
     const Plan p = plan_of(nseq, Hk, page, max_pages, a);
     if (p.wgs >= 1 << 30) return -1;
     return p.nch > 1 ? p.wgs * p.R * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
-    if (mh_kv_prompt(a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
+    if (mh_kv_prompt(type, a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
     const Plan p = plan_of(t.nseq, t.Hk, t.page, t.max_pages, a);
     const StepArgs A{t, a, ws, p.nrt, p.nch, p.R};
     auto go = [&](auto step, auto join) {

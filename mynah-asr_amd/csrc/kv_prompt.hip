@@ -425,22 +425,35 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
     const float *ml = A.part + wgs * RT * DK;
     auto slot = [&](int i) { return (((size_t)i * A.ntile + at) * A.t.Hk + h) * RT + row; };
     float m = -INFINITY;
+#pragma unroll 8
     for (int i = 0; i < nch; i++) m = fmaxf(m, ml[2 * slot(i)]);
     const float mz = m == -INFINITY ? 0.0f : m;
     f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
-    for (int i = 0; i < nch; i++) {
-        const size_t s = slot(i);
-        const float f = exp2f(ml[2 * s] - mz);
-        l += f * ml[2 * s + 1];
-        o += f * *(const f4 *)(A.part + s * DK + d);
+    constexpr int U = 4;   // chunks whose loads are on their way at a time
+    for (int i0 = 0; i0 < nch; i0 += U) {
+        f4 x[U];
+        float2 y[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const size_t s = slot(min(i0 + u, nch - 1));
+            x[u] = *(const f4 *)(A.part + s * DK + d);
+            y[u] = *(const float2 *)(ml + 2 * s);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i0 + u >= nch) break;
+            const float f = __builtin_amdgcn_exp2f(y[u].x - mz);
+            l += f * y[u].y;
+            o += f * x[u];
+        }
     }
     const int rr = rt * RT + row;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     *(f4 *)(A.a.out + (int64_t)(tl.s.r0 + rr / A.a.G) * A.a.ldo + (h * A.a.G + rr % A.a.G) * DK + d) = o * inv;
 }
 
-// The launch's sizes, from the call's. A tile's keys are split into chunks (of 8
+// The launch's sizes, from the call's. A tile's keys are split into chunks (of 2
 // tiles at least) where its row tiles alone would leave the chip's 512 places
 // (two workgroups a CU) empty.
 struct Plan {
@@ -465,7 +478,7 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const 
     int64_t split = 512 / (ntile * Hk);
     if (split < 1) split = 1;
     int64_t ct = (blocks + split - 1) / split;
-    if (ct < 8) ct = 8;
+    if (ct < 2) ct = 2;
     p.ntile = ntile < 1 << 30 ? (int)ntile : 1 << 30;
     p.ct = (int)ct;
     p.nch = (int)((blocks + ct - 1) / ct);
@@ -475,8 +488,11 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const 
 
 }  // namespace
 
-// Measured crossing of the two forms: see mh_launch_kv_attention.
-bool mh_kv_prompt(const KvAttend &a) { return (int64_t)a.max_new * a.G > 64; }
+// More rows of a sequence and K/V head than two tiles of the few-rows form hold (which reads the
+// keys once a tile): 16 requests of 2000 keys, 32 heads on 8, f16, 32 rows 51 us there and 48 here,
+// 48 rows 70 and 52; two of 30000 81 and 88, 115 and 92. f32 caches, on whose MFMA this form pays for its
+// idle rows, from four tiles: 8 heads, 40 rows 113 and 160, 64 rows 150 and 166.
+bool mh_kv_prompt(int type, const KvAttend &a) { return (int64_t)a.max_new * a.G > (type == KV_F32 ? 64 : 32); }
 
 int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     const Plan p = plan_of(nseq, rows, Hk, page, max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
