@@ -4,7 +4,7 @@
 //
 // with causal order, a sliding window and first keys that stay visible decided by
 // position (kv.h). The G query heads that share a K/V head are rows of one
-// product, as are a sequence's new rows: tile rows r = token * G + head, 16 a tile.
+// product, as are a sequence's new rows: tile rows r = token * G + head, 16 NR a tile.
 //
 // One workgroup = four waves = one chunk of the keys that one tile sees, for one
 // K/V head. The keys are a list of blocks of 64 (kv_span); a wave takes every
@@ -33,7 +33,6 @@ namespace {
 
 constexpr int NW = 4, NTH = 64 * NW;
 constexpr int KB = 64;      // keys of a block
-constexpr int RT = 16;      // rows of a tile
 
 // Blocks a wave takes in one chunk of a tile that sees `cnt`: long lists have
 // longer chunks (fewer partial results to join).
@@ -131,25 +130,33 @@ template <typename T, int DK> struct Wave {   // 16 bits
 #pragma unroll
         for (int n = 0; n < NB; n++) s[n] *= sc;
     }
-    // o[e] += V^T P^T: feature VE (4 g + x) + e of the context in element x
-    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE / 2], const f4 (&p)[NB], f4 (&o)[VE]) {
+    // o[i][e] += V^T P^T: feature VE (4 g + x) + e of the context in element x
+    template <int NR>
+    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE / 2], const f4 (&p)[NR][NB],
+                                                   f4 (&o)[NR][VE]) {
 #pragma unroll
         for (int n = 0; n < NB; n += 2) {
             // slots 8 g + j: keys 4 g + j of tile n, then of tile n + 1
-            const float pf[8] = {p[n][0], p[n][1], p[n][2], p[n][3], p[n + 1][0], p[n + 1][1], p[n + 1][2], p[n + 1][3]};
-            v8 pt[X::N];
-            X::split(pf, pt);
+            v8 pt[NR][X::N];
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const float pf[8] = {p[i][n][0],     p[i][n][1],     p[i][n][2],     p[i][n][3],
+                                     p[i][n + 1][0], p[i][n + 1][1], p[i][n + 1][2], p[i][n + 1][3]};
+                X::split(pf, pt[i]);
+            }
 #pragma unroll
             for (int e = 0; e < VE; e++) {
                 uint32_t a[4];
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const int i = n + y / 2, r = 2 * (y & 1);
-                    a[y] = __builtin_amdgcn_perm(v[i][r + 1][e / 2], v[i][r][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+                    const int k = n + y / 2, r = 2 * (y & 1);
+                    a[y] = __builtin_amdgcn_perm(v[k][r + 1][e / 2], v[k][r][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
                 }
                 const v8 av = __builtin_bit_cast(v8, uint4{a[0], a[1], a[2], a[3]});
 #pragma unroll
-                for (int x = 0; x < X::N; x++) o[e] = X::mfma16(av, pt[x], o[e]);
+                for (int x = 0; x < X::N; x++)
+#pragma unroll
+                    for (int i = 0; i < NR; i++) o[i][e] = X::mfma16(av, pt[i][x], o[i][e]);
             }
         }
     }
@@ -184,13 +191,17 @@ template <int DK> struct Wave<float, DK> {
                 for (int n = 0; n < NB; n++) s[n] = mfma4(__uint_as_float(k[n][u][j]), q[j], s[n]);
         }
     }
-    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE], const f4 (&p)[NB], f4 (&o)[VE]) {
+    template <int NR>
+    static __device__ __forceinline__ void context(const uint32_t (&v)[NB][4][VE], const f4 (&p)[NR][NB],
+                                                   f4 (&o)[NR][VE]) {
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll
             for (int x = 0; x < 4; x++)
 #pragma unroll
-                for (int e = 0; e < VE; e++) o[e] = mfma4(__uint_as_float(v[n][x][e]), p[n][x], o[e]);
+                for (int e = 0; e < VE; e++)
+#pragma unroll
+                    for (int i = 0; i < NR; i++) o[i][e] = mfma4(__uint_as_float(v[n][x][e]), p[i][n][x], o[i][e]);
     }
     static __device__ __forceinline__ bool clean(uint32_t &x) {
         const bool odd = !(fabsf(__uint_as_float(x)) < INFINITY);
@@ -201,9 +212,10 @@ template <int DK> struct Wave<float, DK> {
 
 __device__ __attribute__((aligned(16))) const float kv_zeros[128] = {};
 
-template <typename T, int DK>
-__global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
+template <typename T, int DK, int NR>
+__global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs A) {
     using W = Wave<T, DK>;
+    constexpr int RT = 16 * NR;
     constexpr int EL = 16 / sizeof(T);       // features of a 16-byte load
     constexpr int NB = W::NB, NU = W::NU, VE = W::VE;
     constexpr int VB = VE * sizeof(T);       // bytes of a value row, per lane
@@ -212,7 +224,7 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     __shared__ float mls[NW][RT][2];
     // q's fragments, then the waves' contexts
     __shared__ __attribute__((aligned(16))) float os[NW][RT][OS];
-    static_assert(W::QF * 1024 <= sizeof os, "q in LDS");
+    static_assert(NR * W::QF * 1024 <= sizeof os, "q in LDS");
     uint4 *ql = (uint4 *)os + (threadIdx.x & 63);
     const KvTables &t = A.t;
     const KvAttend &a = A.a;
@@ -283,21 +295,29 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
     bool more = seek(e, n0);
     if (more) fetch(n0);
 
-    // this lane's query row, times scale and log2(e)
-    const int r = rt * RT + min(c, tl.live - 1), tok = r / a.G;
-    const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
-    W wv;
-    wv.put_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
-             c < tl.live, g, w, ql);
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f;
-    f4 o[VE];
+    // this lane's query rows (one of each sixteen), times scale and log2(e)
+    int lo[NR], hi[NR];
+    W wv[NR];
+    float m[NR], l[NR];
+    f4 o[NR][VE];
 #pragma unroll
-    for (int x = 0; x < VE; x++) o[x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < NR; i++) {
+        const int r = rt * RT + min(16 * i + c, tl.live - 1), tok = r / a.G;
+        lo[i] = kv_first(a, tl.s, tok);
+        hi[i] = kv_last(t, a, tl.s, tok);
+        wv[i].put_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
+                    16 * i + c < tl.live, g, w, ql + 64 * W::QF * i);
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < VE; x++) o[i][x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __syncthreads();
 
     while (more) {
-        f4 s[NB];
-        wv.scores(ql, kr, s);
+        f4 s[NR][NB];
+#pragma unroll
+        for (int i = 0; i < NR; i++) wv[i].scores(ql + 64 * W::QF * i, kr, s[i]);
         bool odd = false;
         if (part(all, n0) != part(~0ull, 0)) {
             const uint32_t see = part(some, n0) >> (4 * g);
@@ -306,7 +326,10 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const int j = j0 + 16 * (n0 + n) + 4 * g + x;
-                    s[n][x] = (see >> (16 * n + x) & 1) && j <= hi && (j >= lo || j < a.sinks) ? s[n][x] : -INFINITY;
+                    const bool in = see >> (16 * n + x) & 1;
+#pragma unroll
+                    for (int i = 0; i < NR; i++)
+                        s[i][n][x] = in && j <= hi[i] && (j >= lo[i] || j < a.sinks) ? s[i][n][x] : -INFINITY;
                 }
             // A value that only some rows see meets the others' probability 0, which
             // hides it unless it is not finite: such an element counts as 0 in the
@@ -320,38 +343,45 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
                         for (int y = 0; y < VB / 4; y++) odd |= W::clean(vr[n][x][y]);
             }
         }
-        float mx = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < NB; n++)
+        for (int i = 0; i < NR; i++) {
+            float mx = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 4; x++) mx = fmaxf(mx, s[n][x]);
-        const float mn = fmaxf(m, max_g(mx)), mz = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - mz);
-        m = mn;
-        l *= al;
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int n = 0; n < NB; n++)
+                for (int x = 0; x < 4; x++) mx = fmaxf(mx, s[i][n][x]);
+            const float mn = fmaxf(m[i], max_g(mx)), mz = mn == -INFINITY ? 0.0f : mn;
+            const float al = __builtin_amdgcn_exp2f(m[i] - mz);
+            m[i] = mn;
+            l[i] *= al;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                s[n][x] = __builtin_amdgcn_exp2f(s[n][x] - mz + W::TOP);
-                l += s[n][x];
-            }
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int x = 0; x < VE; x++) o[x] *= al;
-        W::context(vr, s, o);
+                for (int x = 0; x < 4; x++) {
+                    s[i][n][x] = __builtin_amdgcn_exp2f(s[i][n][x] - mz + W::TOP);
+                    l[i] += s[i][n][x];
+                }
+#pragma unroll
+            for (int x = 0; x < VE; x++) o[i][x] *= al;
+        }
+        W::template context<NR>(vr, s, o);
         if (__any(odd)) {
             for (int jj = 16 * n0; jj < 16 * (n0 + NB); jj++) {
                 const uint32_t at_v = slots[w][jj];
                 const int j = j0 + jj;
-                if (at_v == KV_NONE || j > hi || (j < lo && j >= a.sinks)) continue;
+                if (at_v == KV_NONE) continue;
                 const T *vp = (const T *)t.v + (size_t)at_v * DK;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+                for (int i = 0; i < NR; i++) {
+                    if (j > hi[i] || (j < lo[i] && j >= a.sinks)) continue;
 #pragma unroll
-                    for (int y = 0; y < VE; y++) {
-                        const float v = (float)vp[VE * (4 * g + x) + y];
-                        if (!(fabsf(v) < INFINITY)) o[y][x] += v;
-                    }
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int y = 0; y < VE; y++) {
+                            const float v = (float)vp[VE * (4 * g + x) + y];
+                            if (!(fabsf(v) < INFINITY)) o[i][y][x] += v;
+                        }
+                }
             }
         }
         n0 += NB;
@@ -359,31 +389,38 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
         more = seek(e, n0);
         if (more) fetch(n0);
     }
-    l = sum_g(l);
 
     // join the waves
-    if (g == 0) mls[w][c][0] = m, mls[w][c][1] = l;
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        l[i] = sum_g(l[i]);
+        if (g == 0) mls[w][16 * i + c][0] = m[i], mls[w][16 * i + c][1] = l[i];
+    }
     __syncthreads();
-    float mb = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NW; i++) mb = fmaxf(mb, mls[i][c][0]);
-    const float mz = mb == -INFINITY ? 0.0f : mb, f = __builtin_amdgcn_exp2f(m - mz);
-    float lb = 0.0f;
+    for (int i = 0; i < NR; i++) {
+        const int row = 16 * i + c;
+        float mb = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NW; i++) lb += mls[i][c][1] * __builtin_amdgcn_exp2f(mls[i][c][0] - mz);
+        for (int k = 0; k < NW; k++) mb = fmaxf(mb, mls[k][row][0]);
+        const float mz = mb == -INFINITY ? 0.0f : mb, f = __builtin_amdgcn_exp2f(m[i] - mz);
+        float lb = 0.0f;
 #pragma unroll
-    for (int x = 0; x < 4; x++)
+        for (int k = 0; k < NW; k++) lb += mls[k][row][1] * __builtin_amdgcn_exp2f(mls[k][row][0] - mz);
 #pragma unroll
-        for (int y = 0; y < VE; y += 4) {
-            f4 u;
+        for (int x = 0; x < 4; x++)
 #pragma unroll
-            for (int z = 0; z < 4; z++) u[z] = o[y + z][x] * f;
-            *(f4 *)(&os[w][c][VE * (4 * g + x) + y]) = u;
+            for (int y = 0; y < VE; y += 4) {
+                f4 u;
+#pragma unroll
+                for (int z = 0; z < 4; z++) u[z] = o[i][y + z][x] * f;
+                *(f4 *)(&os[w][row][VE * (4 * g + x) + y]) = u;
+            }
+        if (w == 0 && g == 0 && nch > 1 && row < tl.live) {
+            float *ml = A.part + (size_t)gridDim.x * A.R * DK + ((size_t)blockIdx.x * A.R + row) * 2;
+            ml[0] = mb;
+            ml[1] = lb;
         }
-    if (w == 0 && g == 0 && nch > 1 && c < tl.live) {
-        float *ml = A.part + (size_t)gridDim.x * A.R * DK + ((size_t)blockIdx.x * A.R + c) * 2;
-        ml[0] = mb;
-        ml[1] = lb;
     }
     __syncthreads();
     for (int i = tid; i < tl.live * (DK / 4); i += NTH) {
@@ -410,9 +447,9 @@ __global__ __launch_bounds__(NTH, 3) void k_kv_step(const StepArgs A) {
 // The chunks of a row, joined in their order: out = sum_c 2^(m_c - M) O_c / sum_c
 // 2^(m_c - M) l_c. One workgroup a row and K/V head; NG groups of lanes take every
 // NG-th chunk, then the groups are added in order.
-template <int DK>
+template <int DK, int NR>
 __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
-    constexpr int LN = DK / 4, NG = NTH / LN;
+    constexpr int RT = 16 * NR, LN = DK / 4, NG = NTH / LN;
     __shared__ float red[NW];
     __shared__ __attribute__((aligned(16))) float os[NG][DK];
     __shared__ float ls[NG];
@@ -480,12 +517,17 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
 
 // The launch's sizes: row tiles of a sequence, chunks of a tile, rows of a partial result.
 struct Plan {
-    int nrt, nch, R;
+    int nr, nrt, nch, R;
     int64_t wgs;
 };
 Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
     Plan p;
     const int64_t rows = (int64_t)a.max_new * a.G;
+    // 17 to 32 rows: one tile of 32 reads the keys once for both halves (two requests of 30000 keys, 8 rows,
+    // 32 heads on 8, f16: 73 -> 64 us; 16 of 2000, 5 rows: 48 -> 41). More, on f32 caches: tiles of 16, which
+    // leave fewer rows idle (40 rows, 8 heads: 113 us, in tiles of 32 133).
+    p.nr = rows > 16 && rows <= 32 ? 2 : 1;
+    const int RT = 16 * p.nr;
     p.nrt = (int)((rows + RT - 1) / RT);
     p.R = rows < RT ? (int)rows : RT;
     const int64_t cap = (int64_t)max_pages * page;
@@ -523,11 +565,8 @@ hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvA
         hipLaunchKernelGGL(join, dim3((unsigned)((int64_t)t.nseq * p.nrt * t.Hk), p.R), dim3(NTH), 0, st, A);
         return hipGetLastError();
     };
-    if (dk == 128)
-        return type == KV_F32 ? go(k_kv_step<float, 128>, k_kv_join<128>)
-               : type == KV_F16 ? go(k_kv_step<_Float16, 128>, k_kv_join<128>)
-                                : go(k_kv_step<__bf16, 128>, k_kv_join<128>);
-    return type == KV_F32 ? go(k_kv_step<float, 64>, k_kv_join<64>)
-           : type == KV_F16 ? go(k_kv_step<_Float16, 64>, k_kv_join<64>)
-                            : go(k_kv_step<__bf16, 64>, k_kv_join<64>);
+#define KV_GO(T, DK) (p.nr == 1 ? go(k_kv_step<T, DK, 1>, k_kv_join<DK, 1>) : go(k_kv_step<T, DK, 2>, k_kv_join<DK, 2>))
+    if (dk == 128) return type == KV_F32 ? KV_GO(float, 128) : type == KV_F16 ? KV_GO(_Float16, 128) : KV_GO(__bf16, 128);
+    return type == KV_F32 ? KV_GO(float, 64) : type == KV_F16 ? KV_GO(_Float16, 64) : KV_GO(__bf16, 64);
+#undef KV_GO
 }

@@ -51,35 +51,81 @@ __device__ __forceinline__ float max_halves(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The sequence and its row tile that tile number `at` of the call is: tiles are
-// numbered sequence by sequence, a sequence's last rows (in causal order the
-// longest) first. false: there are fewer. Every thread of the workgroup takes part.
+// The sequence and its row tile that tile number `at` of the call is. Tiles are numbered
+// in rounds: the last of each sequence (in causal order its longest), then the
+// last but one of each that has two, and so on, so that no long one starts late. With
+// T_b tiles in sequence b, sum_b min(T_b, k) of them come before round k. false: there
+// are fewer. Every thread of the workgroup takes part.
+__device__ __forceinline__ int wave_sum_i(int x) {
+    auto step = [&](auto ctrl) { x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, false); };
+    step(std::integral_constant<int, 0xB1>{});    // (the steps of wave_sum)
+    step(std::integral_constant<int, 0x4E>{});
+    step(std::integral_constant<int, 0x141>{});
+    step(std::integral_constant<int, 0x140>{});
+    auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = r[0] + r[1];
+    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return r[0] + r[1];
+}
+__device__ __forceinline__ int block_sum(int x, int *lds) {
+    x = wave_sum_i(x);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
 __device__ __forceinline__ bool find_tile(const KvTables &t, const KvAttend &a, int at, int &b, int &rt) {
-    __shared__ int sum[NW], hit[2];
+    __shared__ int lds[NW], hit[2];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    for (int base = 0, b0 = 0; b0 < t.nseq; b0 += NTH) {
-        int n = 0;
-        if (b0 + tid < t.nseq) n = (kv_rows(a, kv_seq(t, b0 + tid)) + RT - 1) / RT;
-        int x = n;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-            const int y = __shfl_up(x, m, 64);
-            if (lane >= m) x += y;
-        }
-        if (lane == 63) sum[w] = x;
+    auto tiles = [&](int s) { return s < t.nseq ? (kv_rows(a, kv_seq(t, s)) + RT - 1) / RT : 0; };
+    if (t.nseq == 1) {
+        b = 0;
+        rt = tiles(0) - 1 - at;
+        return rt >= 0;
+    }
+    // up to 64 sequences: each wave by itself, a sequence a lane
+    const bool few = t.nseq <= 64;
+    const int mine = tiles(few ? lane : tid);   // (the others, if there are more, are read again each time)
+    auto before = [&](int k) {
+        if (few) return wave_sum_i(min(mine, k));
+        int x = min(mine, k);
+        for (int s = tid + NTH; s < t.nseq; s += NTH) x += min(tiles(s), k);
+        return block_sum(x, lds);
+    };
+    // the round: the largest k with before(k) <= at
+    int k = 0, top = (int)(((int64_t)a.max_new * a.G + RT - 1) / RT), base = 0;
+    while (k < top) {
+        const int mid = k + (top - k + 1) / 2, n = before(mid);
+        if (n <= at) k = mid, base = n;
+        else top = mid - 1;
+    }
+    // in it, the sequences that have more than k tiles, in order
+    at -= base;
+    if (few) {
+        const uint64_t have = __ballot(mine > k);
+        const uint64_t here = __ballot(mine > k && __popcll(have & ((1ull << lane) - 1)) == at);
+        if (!here) return false;
+        b = __ffsll((unsigned long long)here) - 1;
+        rt = __shfl(mine, b, 64) - 1 - k;
+        return true;
+    }
+    for (int s0 = 0; s0 < t.nseq; s0 += NTH) {
+        const int n = s0 ? tiles(s0 + tid) : mine;
+        const uint64_t have = __ballot(n > k);
+        __syncthreads();
+        if (lane == 0) lds[w] = __popcll(have);
         if (tid == 0) hit[0] = -1;
         __syncthreads();
-        int before = base + x - n;
-        for (int i = 0; i < w; i++) before += sum[i];
-        if (at >= before && at < before + n) hit[0] = b0 + tid, hit[1] = n - 1 - (at - before);
-        for (int i = 0; i < NW; i++) base += sum[i];
+        int rank = __popcll(have & ((1ull << lane) - 1));
+        for (int i = 0; i < w; i++) rank += lds[i];
+        if (n > k && rank == at) hit[0] = s0 + tid, hit[1] = n - 1 - k;
+        at -= lds[0] + lds[1] + lds[2] + lds[3];
         __syncthreads();
         if (hit[0] >= 0) {
             b = hit[0];
             rt = hit[1];
             return true;
         }
-        __syncthreads();
     }
     return false;
 }
