@@ -311,6 +311,11 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     const int r = 32 * w + c, tok = (rt * RT + min(r, tl.live - 1)) / a.G;
     const int head = h * a.G + (rt * RT + min(r, tl.live - 1)) % a.G;
     const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
+    // what the wave's first and last row see (a wave of no rows: nothing)
+    const bool idle = 32 * w >= tl.live;
+    const int t0 = (rt * RT + min(32 * w, tl.live - 1)) / a.G, t1 = (rt * RT + min(32 * w + 31, tl.live - 1)) / a.G;
+    const int wlo0 = kv_first(a, tl.s, t0), wlo1 = kv_first(a, tl.s, t1);
+    const int whi0 = kv_last(t, a, tl.s, t0), whi1 = idle ? -1 : kv_last(t, a, tl.s, t1);
     W wv;
     wv.init(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + head * DK, a.scale * 1.4426950408889634f, r < tl.live, lane);
     f16v o[DT];
@@ -356,17 +361,22 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         // product and is added afterwards to the rows that see it.
         int odd = 0;
         if (!all) {
-            for (int i = tid; i < TB / 4; i += NTH) {
-                uint32_t x = ((uint32_t *)vt)[i];
-                if (W::clean(x)) {
+#pragma unroll
+            for (int i = 0; i < TB / 16 / NTH; i++) {
+                uint4 x = ((uint4 *)vt)[tid + NTH * i];
+                const bool y[4] = {W::clean(x.x), W::clean(x.y), W::clean(x.z), W::clean(x.w)};
+                if (y[0] || y[1] || y[2] || y[3]) {
                     odd = 1;
-                    ((uint32_t *)vt)[i] = x;
+                    ((uint4 *)vt)[tid + NTH * i] = x;
                 }
             }
             odd = __syncthreads_or(odd);
         }
+        if (j0 > whi1 || (j0 + KT <= wlo0 && j0 >= a.sinks)) return;   // no row of this wave sees any
+        const bool every = __builtin_amdgcn_readfirstlane(okw == (Word)~0ull && j0 + KT - 1 <= whi0 &&
+                                                          (j0 >= wlo1 || j0 + KT <= a.sinks));
         wv.tile(kt, vt, ka, va, o, [&](int n, f16v &s, float sc) {
-            if (!all) {
+            if (!every) {
                 const uint32_t mine = (uint32_t)(okw >> (32 * n + 4 * hf));
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
