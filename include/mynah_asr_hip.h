@@ -353,12 +353,14 @@ enum {
 };
 
 /* The pool. Key (or value) of cache slot s of a page and head h: the head_dim
- * elements at [page][h][s][0]. */
+ * elements at [page][h][s][0]. n_pages * n_kv_heads * page_size stays below
+ * 2^32 - 1. The calls run on the current device: stream and buffers on another
+ * one are refused. */
 typedef struct {
     int type;         /* MYNAH_ASR_HIP_F32, _F16 or _BF16 */
     int n_pages;
     int page_size;    /* slots of a page, any number from 1 */
-    int n_kv_heads;
+    int n_kv_heads;   /* up to 65536 */
     int head_dim;     /* 64 or 128 */
     void *k, *v;      /* device, [n_pages][n_kv_heads][page_size][head_dim] each, 16-byte aligned */
 } mynah_asr_hip_kv_cache;
@@ -377,7 +379,7 @@ typedef struct {
  * over. */
 typedef struct {
     int nseq;              /* sequences, up to 65535 */
-    int rows;              /* rows of the activation buffers, up to 2^24; those from
+    int rows;              /* rows of the activation buffers, below 2^24; those from
                               row_start[nseq] on are left as they are */
     int max_pages;         /* row length of `pages` */
     int max_new;           /* most rows of one sequence */
@@ -422,13 +424,15 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
  * n_heads heads, ldq / ldo floats apart, 16-byte aligned, strides multiples of
  * 4; out may be q (ldo = ldq), and may not overlap it otherwise.
  *
- * Products and sums as f32: |out - ref| <= 1e-5 * max|v| over the keys a row
- * sees, for finite scores that differ by less than 2^20. A row's bits depend on
- * its q, the keys and values it sees, its position, and the call's sizes
- * and settings; keys and values it does not see (hidden, behind len[b], in the
- * rest of a page) change nothing, NaN and infinity included. A row that sees a
- * NaN or an infinity gives NaN or infinity where f32 arithmetic does, or NaN where
- * it gives infinity.
+ * Products and sums as f32 ones: for finite inputs |out - ref| <= 2^-24 max|v|
+ * (2 (head_dim + 8) A + n / 8 + 300), A the largest sum of |scale q k| over the n
+ * keys a row sees (a bound; the relative error measures 5e-7 to 1.2e-6). A row's bits
+ * depend on its q, the keys and values it sees, its position, its place among its
+ * sequence's new rows and their number, and the call's sizes and settings; up to 32
+ * rows (max_new * n_heads / n_kv_heads), not on nseq either. Keys and values that it
+ * does not see (hidden, behind len[b], in the rest of a page) change nothing, NaN
+ * and infinity included. A row that sees a NaN or an infinity gives what f32
+ * arithmetic gives or NaN: a key's in the whole head, a value's in its feature alone.
  *
  * ws: device workspace of ws_bytes, 16-byte aligned, at least
  * mynah_asr_hip_kv_attention_ws_bytes; NULL: the calling thread's own, grown as

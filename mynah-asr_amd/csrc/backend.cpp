@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -1135,7 +1136,7 @@ int subsampling_dev(Ctx *c, const mynah_asr_hip_subsampling *ss, const float *fe
 // The paged key-value cache. Arguments are checked before the device is
 // looked for, so a wrong call is refused the same way everywhere.
 
-constexpr int kKvRows = 1 << 24, kKvLen = 1 << 30, kKvSeqs = 65535;
+constexpr int kKvRows = (1 << 24) - 1, kKvLen = 1 << 30, kKvSeqs = 65535;
 
 int kv_type(int type) {
     return type == MYNAH_ASR_HIP_F32 ? KV_F32 : type == MYNAH_ASR_HIP_F16 ? KV_F16 : type == MYNAH_ASR_HIP_BF16 ? KV_BF16 : -1;
@@ -1147,10 +1148,11 @@ int kv_sizes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
     if (kv_type(c->type) < 0) return fail("cache type must be F32, F16 or BF16");
     if (c->head_dim != 64 && c->head_dim != 128) return fail("head size must be 64 or 128");
     if (c->n_pages <= 0 || c->page_size <= 0 || c->n_kv_heads <= 0) return fail("bad argument: an empty cache");
+    if (c->n_kv_heads > 65536) return fail("n_kv_heads must be at most 65536");
     if ((double)c->n_pages * c->page_size * c->n_kv_heads >= 4294967295.0)
         return fail("cache: n_pages * page_size * n_kv_heads must stay below 2^32 - 1");
     if (b->nseq < 0 || b->nseq > kKvSeqs) return fail("batch: nseq must be 0 to 65535");
-    if (b->rows < 0 || b->rows > kKvRows) return fail("batch: rows must be 0 to 2^24");
+    if (b->rows < 0 || b->rows > kKvRows) return fail("batch: rows must be 0 to 2^24 - 1");
     if (b->max_pages < 0 || b->max_new < 0 || b->max_len < 0 || b->max_len > kKvLen)
         return fail("batch: max_pages, max_new and max_len (up to 2^30) may not be negative");
     return 0;
@@ -1173,8 +1175,14 @@ int kv_pointers(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b
     return 0;
 }
 
-// The kernels run on the current device: its stream, its memory.
-int kv_device(const void *pool, hipStream_t st) {
+// The kernels run on the current device: its stream, its memory (ptrs, null ones passed over). Where
+// there is one device there is nothing to ask.
+int kv_device(hipStream_t st, std::initializer_list<const void *> ptrs) {
+    static const int devices = [] {
+        int n = 0;
+        return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
+    }();
+    if (devices <= 1) return 0;
     int cur = 0;
     hipDevice_t sd = 0;
     if (hipGetDevice(&cur) != hipSuccess) return fail("no current device");
@@ -1183,12 +1191,15 @@ int kv_device(const void *pool, hipStream_t st) {
     } else {
         (void)hipGetLastError();
     }
-    hipPointerAttribute_t at;
-    if (hipPointerGetAttributes(&at, pool) == hipSuccess) {
+    for (const void *p : ptrs) {
+        hipPointerAttribute_t at;
+        if (!p) continue;
+        if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+            (void)hipGetLastError();
+            continue;
+        }
         if (at.type == hipMemoryTypeDevice && at.device != cur)
-            return fail("the cache lies on another device than the current one");
-    } else {
-        (void)hipGetLastError();
+            return fail("a buffer lies on another device than the current one");
     }
     return 0;
 }
@@ -1442,6 +1453,7 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
     if (kv_sizes(c, b) || kv_pointers(c, b)) return -1;
     const int dk = c->head_dim;
     if (n_heads < 0 || n_heads > 65536) return fail("n_heads must be 0 to 65536");
+    if (!n_heads) q = nullptr, q_out = nullptr;
     if (n_heads && (kv_rows("q", q, ldq, (int64_t)n_heads * dk) || kv_rows("q_out", q_out, ldqo, (int64_t)n_heads * dk)))
         return -1;
     if (kv_rows("k", k, ldk, (int64_t)c->n_kv_heads * dk) || kv_rows("v", v, ldv, (int64_t)c->n_kv_heads * dk)) return -1;
@@ -1459,7 +1471,7 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
     Ctx *x;
     if (begin(&x)) return -1;
     hipStream_t st = pick_stream(stream);
-    if (kv_device(c->k, st)) return -1;
+    if (kv_device(st, {c->k, c->v, b->row_start, b->len, b->pages, q, q_out, k, v, a.qn, a.kn, a.freq})) return -1;
     if (b->rows == 0 || b->nseq == 0) return 0;
     hipError_t e = mh_launch_kv_append(kv_tables(c, b), kv_type(c->type), dk, a, st);
     return e == hipSuccess ? 0 : fail("append launch failed", hipGetErrorString(e));
@@ -1503,7 +1515,7 @@ int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_
     Ctx *x;
     if (begin(&x)) return -1;
     hipStream_t st = pick_stream(stream);
-    if (kv_device(c->k, st)) return -1;
+    if (kv_device(st, {c->k, c->v, b->row_start, b->len, b->pages, q, out, ws})) return -1;
     if (none) return 0;
     if (!ws && need) {
         note_capture(st);   // the thread's workspace may grow

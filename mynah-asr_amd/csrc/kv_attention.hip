@@ -51,8 +51,8 @@ int most_chunks(int n) {
 struct StepArgs {
     KvTables t;
     KvAttend a;
-    float *part;      // partial contexts [workgroup][R][DK], then their maxima and sums [workgroup][R][2]
-    int nrt, nch, R;  // row tiles of a sequence, chunks of a tile (at most), rows of a partial result
+    float *part;   // partial contexts [workgroup][R][DK], then their maxima and sums [workgroup][R][2]
+    int nch, R;    // chunks of a sequence's keys (at most), rows of a partial result
 };
 
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -233,10 +233,8 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
     int at = blockIdx.x;
     const int h = at % t.Hk;
     at /= t.Hk;
-    const int rt = at % A.nrt;   // (the tiles that read the same keys run together, on one XCD where Hk is a multiple of 8)
-    at /= A.nrt;
     const int ch = at % A.nch, b = at / A.nch;
-    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
+    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, 0);
     if (tl.live <= 0) return;
     const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
     if (ch >= nch) return;
@@ -302,7 +300,7 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
     f4 o[NR][VE];
 #pragma unroll
     for (int i = 0; i < NR; i++) {
-        const int r = rt * RT + min(16 * i + c, tl.live - 1), tok = r / a.G;
+        const int r = min(16 * i + c, tl.live - 1), tok = r / a.G;
         lo[i] = kv_first(a, tl.s, tok);
         hi[i] = kv_last(t, a, tl.s, tok);
         wv[i].put_q(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + (h * a.G + r % a.G) * DK, a.scale * 1.4426950408889634f,
@@ -438,9 +436,8 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
         ms = ms == -INFINITY ? 0.0f : ms;
 #pragma unroll
         for (int k = 0; k < NW; k++) ls += mls[k][row][1] * __builtin_amdgcn_exp2f(mls[k][row][0] - ms);
-        const int rr = rt * RT + row;
         const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-        *(f4 *)(a.out + (int64_t)(tl.s.r0 + rr / a.G) * a.ldo + (h * a.G + rr % a.G) * DK + d) = u * inv;
+        *(f4 *)(a.out + (int64_t)(tl.s.r0 + row / a.G) * a.ldo + (h * a.G + row % a.G) * DK + d) = u * inv;
     }
 }
 
@@ -454,19 +451,16 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
     __shared__ __attribute__((aligned(16))) float os[NG][DK];
     __shared__ float ls[NG];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.y;
-    int at = blockIdx.x;
-    const int h = at % A.t.Hk;
-    at /= A.t.Hk;
-    const int rt = at % A.nrt, b = at / A.nrt;
-    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, rt);
+    const int h = blockIdx.x % A.t.Hk, b = blockIdx.x / A.t.Hk;
+    const KvTile tl = kv_tile<RT, KB>(A.t, A.a, b, 0);
     if (row >= tl.live) return;
     const int nch = chunks_of(tl.sp.cnt);
     if (nch <= 1) return;
-    // chunk i's workgroup: ((b nch_max + i) nrt + rt) Hk + h
-    const size_t wg0 = ((size_t)b * A.nch * A.nrt + rt) * A.t.Hk + h;
-    const size_t wgs = (size_t)A.t.nseq * A.nrt * A.nch * A.t.Hk;
+    // chunk i's workgroup: (b nch_max + i) Hk + h
+    const size_t wg0 = (size_t)b * A.nch * A.t.Hk + h;
+    const size_t wgs = (size_t)A.t.nseq * A.nch * A.t.Hk;
     const float *ml = A.part + wgs * A.R * DK;
-    auto slot = [&](int i) { return (wg0 + (size_t)i * A.nrt * A.t.Hk) * A.R + row; };
+    auto slot = [&](int i) { return (wg0 + (size_t)i * A.t.Hk) * A.R + row; };
     // the first contexts are on their way while the maximum is found
     constexpr int U = 4;
     const int gi = tid / LN, d = 4 * (tid % LN);
@@ -509,38 +503,32 @@ __global__ __launch_bounds__(NTH) void k_kv_join(const StepArgs A) {
             o += *(const f4 *)&os[i][d];
             l += ls[i];
         }
-        const int rr = rt * RT + row;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *(f4 *)(A.a.out + (int64_t)(tl.s.r0 + rr / A.a.G) * A.a.ldo + (h * A.a.G + rr % A.a.G) * DK + d) = o * inv;
+        *(f4 *)(A.a.out + (int64_t)(tl.s.r0 + row / A.a.G) * A.a.ldo + (h * A.a.G + row % A.a.G) * DK + d) = o * inv;
     }
 }
 
-// The launch's sizes: row tiles of a sequence, chunks of a tile, rows of a partial result.
+// The launch's sizes: sixteens of rows in a tile (17 to 32 rows in one tile read the keys once: two requests
+// of 30000 keys, 8 rows, 32 heads on 8, f16, 64 us, in two tiles 73; 16 of 2000, 5 rows, 41 and 48),
+// chunks of a sequence's keys, rows of a partial result.
 struct Plan {
-    int nr, nrt, nch, R;
+    int nr, nch, R;
     int64_t wgs;
 };
 Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
     Plan p;
-    const int64_t rows = (int64_t)a.max_new * a.G;
-    // 17 to 32 rows: one tile of 32 reads the keys once for both halves (two requests of 30000 keys, 8 rows,
-    // 32 heads on 8, f16: 73 -> 64 us; 16 of 2000, 5 rows: 48 -> 41). More, on f32 caches: tiles of 16, which
-    // leave fewer rows idle (40 rows, 8 heads: 113 us, in tiles of 32 133).
-    p.nr = rows > 16 && rows <= 32 ? 2 : 1;
-    const int RT = 16 * p.nr;
-    p.nrt = (int)((rows + RT - 1) / RT);
-    p.R = rows < RT ? (int)rows : RT;
+    p.R = a.max_new * a.G;   // (at most 32)
+    p.nr = p.R > 16 ? 2 : 1;
     const int64_t cap = (int64_t)max_pages * page;
     const int keys = (int)(a.max_len < cap ? a.max_len : cap), all = (keys + KB - 1) / KB;
     int64_t blocks = all;
     if (a.window) {
-        // a tile's rows are up to ceil(16 / G) tokens apart; each end of each part may cut a block
-        const int64_t toks = (RT + a.G - 1) / a.G + 1;
-        const int64_t win = ((int64_t)a.window + toks + KB - 1) / KB + 1, sink = ((int64_t)a.sinks + KB - 1) / KB + 1;
+        // (a sequence's rows reach max_new - 1 keys further; each end of each part may cut a block)
+        const int64_t win = ((int64_t)a.window + a.max_new + KB - 1) / KB + 1, sink = ((int64_t)a.sinks + KB - 1) / KB + 1;
         if (win + sink < blocks) blocks = win + sink;
     }
     p.nch = most_chunks((int)blocks);
-    p.wgs = (int64_t)nseq * p.nrt * p.nch * Hk;
+    p.wgs = (int64_t)nseq * p.nch * Hk;
     return p;
 }
 
@@ -548,21 +536,21 @@ Plan plan_of(int nseq, int Hk, int page, int max_pages, const KvAttend &a) {
 
 int64_t mh_kv_attention_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     if ((int64_t)a.max_new * a.G >= 1 << 30) return -1;
-    if (mh_kv_prompt(type, a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, type, dk, a);
+    if (mh_kv_prompt(a)) return mh_kv_prompt_ws(nseq, rows, Hk, page, max_pages, type, dk, a);
     const Plan p = plan_of(nseq, Hk, page, max_pages, a);
-    if (p.wgs >= 1 << 30) return -1;
+    if (p.wgs >= 1 << 24) return -1;   // (a launch holds less than 2^32 threads)
     return p.nch > 1 ? p.wgs * p.R * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
-    if (mh_kv_prompt(type, a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
+    if (mh_kv_prompt(a)) return mh_launch_kv_prompt(t, type, dk, a, ws, st);
     const Plan p = plan_of(t.nseq, t.Hk, t.page, t.max_pages, a);
-    const StepArgs A{t, a, ws, p.nrt, p.nch, p.R};
+    const StepArgs A{t, a, ws, p.nch, p.R};
     auto go = [&](auto step, auto join) {
         hipLaunchKernelGGL(step, dim3((unsigned)p.wgs), dim3(NTH), 0, st, A);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || p.nch <= 1) return e;
-        hipLaunchKernelGGL(join, dim3((unsigned)((int64_t)t.nseq * p.nrt * t.Hk), p.R), dim3(NTH), 0, st, A);
+        hipLaunchKernelGGL(join, dim3((unsigned)((int64_t)t.nseq * t.Hk), p.R), dim3(NTH), 0, st, A);
         return hipGetLastError();
     };
 #define KV_GO(T, DK) (p.nr == 1 ? go(k_kv_step<T, DK, 1>, k_kv_join<DK, 1>) : go(k_kv_step<T, DK, 2>, k_kv_join<DK, 2>))

@@ -12,10 +12,14 @@
 // B column c, D rows 8 (e / 4) + 4 hf + e % 4, column c): a lane holds the scores of
 // one query row, half of a tile's keys, and its probabilities are the second
 // product's B operand as they lie, which is free to take its keys in that order.
-//   16 bits: the 32x32x16 MFMA of the cache's type, slots 8 hf + j; value rows come
-//     transposed from LDS (ds_read_b64_tr_b16); q and probabilities in terms
-//     (kv_terms.h; a q row scaled by a power of two, probabilities below 2^14).
-//   f32: the 32x32x2 f32 MFMA, slot hf.
+// The 32x32x16 MFMA of 16-bit types, slots 8 hf + j; value rows come transposed from
+// LDS (ds_read_b64_tr_b16); q and probabilities in terms (kv_terms.h; for f16 a q row scaled
+// by a power of two, probabilities below 2^14).
+//   f32 caches: a tile is taken apart into three bf16 planes in LDS, exactly (8 bits
+//   each); six of the nine products of terms, all but those below 2^-24 of the whole.
+//   The copies of the next tile run into the one f32 slot while the planes are in use.
+//   (The 32x32x2 f32 MFMA takes 2.7 times as long: four prompts with a window of 512,
+//   8 heads, 214 us, now 128.)
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
 // is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + 8).
 #include <hip/hip_runtime.h>
@@ -55,7 +59,8 @@ __device__ __forceinline__ float max_halves(float x) {
 // in rounds: the last of each sequence (in causal order its longest), then the
 // last but one of each that has two, and so on, so that no long one starts late. With
 // T_b tiles in sequence b, sum_b min(T_b, k) of them come before round k. false: there
-// are fewer. Every thread of the workgroup takes part.
+// are fewer. Every thread of the workgroup takes part; lds: NW + 2 words, free again
+// after the workgroup's next barrier.
 __device__ __forceinline__ int wave_sum_i(int x) {
     auto step = [&](auto ctrl) { x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, false); };
     step(std::integral_constant<int, 0xB1>{});    // (the steps of wave_sum)
@@ -74,8 +79,8 @@ __device__ __forceinline__ int block_sum(int x, int *lds) {
     __syncthreads();
     return lds[0] + lds[1] + lds[2] + lds[3];
 }
-__device__ __forceinline__ bool find_tile(const KvTables &t, const KvAttend &a, int at, int &b, int &rt) {
-    __shared__ int lds[NW], hit[2];
+__device__ __forceinline__ bool find_tile(const KvTables &t, const KvAttend &a, int at, int *lds, int &b, int &rt) {
+    int *hit = lds + NW;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     auto tiles = [&](int s) { return s < t.nseq ? (kv_rows(a, kv_seq(t, s)) + RT - 1) / RT : 0; };
     if (t.nseq == 1) {
@@ -237,44 +242,74 @@ template <typename T, int DK> struct Ops {   // 16 bits
         return l || h;
     }
 };
-template <int DK> struct Ops<float, DK> {
-    static constexpr int KS = DK / 8, DT = DK / 32, ROW = DK * 4;
-    static __device__ __forceinline__ int swz(int row) { return row & 15; }   // (of any 16 rows one piece each, in all banks)
-    static __device__ __forceinline__ int feature(int d, int x, int hf) { return DT * (8 * (x / 4) + 4 * hf + x % 4) + d; }
-    float q[KS][4];
-    int at_k, at_v;
-    __device__ __forceinline__ void init(const float *qp, float f, bool live, int lane) {
-        const int c = lane & 31, hf = lane >> 5;
-        at_k = c * ROW + (hf ^ swz(c)) * 16;
-        at_v = 4 * hf * ROW + ((DT * c / 4) ^ swz(4 * hf)) * 16 + DT * c % 4 * 4;
+// f32: bf16's operands, a tile's planes behind each other
+template <int DK> struct Ops<float, DK> : Ops<__bf16, DK> {
+    using B = Ops<__bf16, DK>;
+    using X = typename B::X;
+    typedef typename B::v8 v8;
+    static constexpr int KS = B::KS, DT = B::DT, ROW = B::ROW, PLANE = KB<float> * ROW;
+    // sum += a b, a and b of three terms each
+    static __device__ __forceinline__ f16v product(const v8 (&a)[3], const v8 (&b)[3], f16v sum) {
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const f4 x = *(const f4 *)(qp + 8 * s + 4 * hf);
+        for (int i = 0; i < 3; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) q[s][j] = live ? x[j] * f : 0.0f;
-        }
+            for (int j = 0; j < 3 - i; j++) sum = X::mfma32(a[i], b[j], sum);
+        return sum;
     }
     template <typename F>
     __device__ __forceinline__ void tile(const uint8_t *kt, const uint8_t *vt, int ka, int va, f16v (&o)[DT], F soft) const {
         f16v s = zero16();
 #pragma unroll
         for (int u = 0; u < KS; u++) {
-            const f4 k = *(const f4 *)(kt + (ka ^ 32 * u));
+            v8 k[3];
 #pragma unroll
-            for (int j = 0; j < 4; j++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[u][j], s, 0, 0, 0);
+            for (int i = 0; i < 3; i++) k[i] = *(const v8 *)(kt + i * PLANE + (ka ^ 32 * u));
+            s = product(k, this->q[u], s);
         }
         soft(0, s, 1.0f);
 #pragma unroll
-        for (int x = 0; x < 16; x++) {   // slot hf: key 8 (x / 4) + 4 hf + x % 4, features DT c ..
-            typedef float fd __attribute__((ext_vector_type(DT)));
-            const fd v = *(const fd *)(vt + (8 * (x / 4) + x % 4) * ROW + (va ^ (8 * (x / 4 & 1) + x % 4) * 16));
+        for (int g = 0; g < 2; g++) {
+            float p[8];
 #pragma unroll
-            for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d], s[x], o[d], 0, 0, 0);
+            for (int x = 0; x < 8; x++) p[x] = s[8 * g + x];
+            v8 pt[3];
+            X::split(p, pt);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                v8 v[3];
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    s4 y[2];
+#pragma unroll
+                    for (int z = 0; z < 2; z++)
+                        y[z] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s4 *)(vt + i * PLANE + (16 * g + 8 * z) * ROW + (va ^ (64 * d + 32 * z))));
+                    v[i] = __builtin_bit_cast(v8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                o[d] = product(v, pt, o[d]);
+            }
         }
     }
-    static __device__ __forceinline__ bool clean(uint32_t &x) {
-        const bool odd = !(fabsf(__uint_as_float(x)) < INFINITY);
-        x = odd ? 0u : x;
+    // eight elements into their place in the three planes: 8 bits of each, cut off
+    static __device__ __forceinline__ void put(float (&x)[8], uint8_t *at) {
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t a = __float_as_uint(x[2 * j]), b = __float_as_uint(x[2 * j + 1]);
+                h[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                if (i < 2) {
+                    x[2 * j] -= __uint_as_float(a & 0xffff0000u);
+                    x[2 * j + 1] -= __uint_as_float(b & 0xffff0000u);
+                }
+            }
+            *(uint4 *)(at + i * PLANE) = uint4{h[0], h[1], h[2], h[3]};
+        }
+    }
+    static __device__ __forceinline__ bool clean(float &x) {
+        const bool odd = !(fabsf(x) < INFINITY);
+        x = odd ? 0.0f : x;
         return odd;
     }
 };
@@ -282,15 +317,16 @@ template <int DK> struct Ops<float, DK> {
 template <typename T, int DK>
 __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     using W = Ops<T, DK>;
+    constexpr bool F32 = sizeof(T) == 4;
     constexpr int DT = W::DT, KT = KB<T>;
-    constexpr int CH = W::ROW / 16;                // 16-byte pieces of a row
-    constexpr int TB = KT * W::ROW;                // bytes of a tile
+    constexpr int ROW = DK * sizeof(T), CH = ROW / 16;   // bytes of a row of the cache, 16-byte pieces
+    constexpr int TB = KT * ROW;                   // bytes of a tile
     constexpr int WR = KT / NW;                    // rows of a tile that a wave copies
     constexpr int RPI = 64 / CH;                   // rows of one copy instruction
-    __shared__ __attribute__((aligned(16))) uint8_t k0[TB], k1[TB], v0[TB], v1[TB];
-    typedef typename std::conditional<KT == 64, uint16_t, uint8_t>::type Bits;   // one a row that a wave copies
-    typedef typename std::conditional<KT == 64, uint64_t, uint32_t>::type Word;
-    __shared__ __attribute__((aligned(8))) Bits valid[2][NW];
+    // (Separate arrays, so that reads of one do not wait for copies into another. f32: one slot and
+    // the planes; with heads of 128 that is just half of a CU's LDS, so there is no other array.)
+    __shared__ __attribute__((aligned(16))) uint8_t k0[TB], k1[F32 ? 16 : TB], v0[TB], v1[F32 ? 16 : TB];
+    __shared__ __attribute__((aligned(16))) uint8_t kp[F32 ? 3 * KT * DK * 2 : 16], vp[F32 ? 3 * KT * DK * 2 : 16];
     const KvTables &t = A.t;
     const KvAttend &a = A.a;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
@@ -299,7 +335,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     const int h = at % t.Hk;
     at /= t.Hk;
     int b, rt;
-    if (!find_tile(t, a, at % A.ntile, b, rt)) return;
+    if (!find_tile(t, a, at % A.ntile, (int *)k0, b, rt)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     rt = __builtin_amdgcn_readfirstlane(rt);
     const KvTile tl = kv_tile<RT, KT>(t, a, b, rt);
@@ -323,58 +359,44 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     for (int d = 0; d < DT; d++) o[d] = zero16();
     float m = -INFINITY, l = 0.0f;
 
-    // Wave w copies rows WR w .. of a tile; its lanes 0 .. WR - 1 (and again from WR on)
-    // hold their pages, read from the table a tile ahead and looked at when they are used.
-    const int lrow = WR * w + lane % WR;
+    // A lane holds the page of one row of a tile, read from the table a tile ahead and
+    // looked at when it is used; wave w copies rows WR w .. of it.
     auto page_of = [&](int e) {
-        const int j = min(tl.sp.block(min(e, e1 - 1)) * KT + lrow, tl.hi1);
+        const int j = min(tl.sp.block(min(e, e1 - 1)) * KT + lane % KT, tl.hi1);
         return t.pages[(size_t)b * t.max_pages + j / t.page];
     };
-    auto copy = [&](int e, int pg, uint8_t *kd, uint8_t *vd, Bits *ok) {
-        const int j = tl.sp.block(e) * KT + lrow;
+    // copies tile e; which of its rows there are
+    auto copy = [&](int e, int pg, uint8_t *kd, uint8_t *vd) {
+        const int j = tl.sp.block(e) * KT + lane % KT;
         const bool have = j <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
         const uint32_t sl = have ? ((uint32_t)pg * t.Hk + h) * t.page + j % t.page : 0;
-        const uint64_t ball = __ballot(have) & ((1u << WR) - 1);
-        if (lane == 0) ok[w] = (Bits)ball;
 #pragma unroll
         for (int i = 0; i < WR / RPI; i++) {
-            const int rr = RPI * i + lane / CH;
-            const size_t off = (size_t)(uint32_t)__shfl((int)sl, rr, 64) * W::ROW + (((lane % CH) ^ W::swz(WR * w + rr)) * 16);
+            const int rr = WR * w + RPI * i + lane / CH;
+            const size_t off = (size_t)(uint32_t)__shfl((int)sl, rr, 64) * ROW + (((lane % CH) ^ (F32 ? 0 : W::swz(rr))) * 16);
             __builtin_amdgcn_global_load_lds((const glob_void *)((const uint8_t *)t.k + off),
-                                             (lds_void *)(kd + (WR * w + RPI * i) * W::ROW), 16, 0, 0);
+                                             (lds_void *)(kd + (WR * w + RPI * i) * ROW), 16, 0, 0);
             __builtin_amdgcn_global_load_lds((const glob_void *)((const uint8_t *)t.v + off),
-                                             (lds_void *)(vd + (WR * w + RPI * i) * W::ROW), 16, 0, 0);
+                                             (lds_void *)(vd + (WR * w + RPI * i) * ROW), 16, 0, 0);
         }
+        return (uint64_t)__ballot(have);
+    };
+    auto whole = [&](uint64_t ok, int j0, int hi_first, int lo_last) -> bool {   // every row sees every key
+        return __builtin_amdgcn_readfirstlane(ok == ~0ull && j0 + KT - 1 <= hi_first && (j0 >= lo_last || j0 + KT <= a.sinks));
     };
 
-    auto tile = [&](int e, const uint8_t *kt, uint8_t *vt, const Bits *ok) {
+    // Tile e's products. A value that only some rows see meets the others' probability 0,
+    // which hides it unless it is not finite: such an element counts as 0 in the
+    // product (and `odd` says that there are any), and is added afterwards to the rows
+    // that see it.
+    auto tile = [&](int e, uint64_t okw, const uint8_t *kt, const uint8_t *vt, bool odd) {
+        const int j0 = tl.sp.block(e) * KT;
+        if (j0 > whi1 || (j0 + KT <= wlo0 && j0 >= a.sinks)) return;   // no row of this wave sees any
         // (opaque: the addresses formed from these, kept for every tile, would cost
         // registers that the products need)
         int ka = wv.at_k, va = wv.at_v;
         asm volatile("" : "+v"(ka), "+v"(va));
-        const int j0 = tl.sp.block(e) * KT;
-        const Word okw = *(const Word *)ok;
-        const bool all = __builtin_amdgcn_readfirstlane(okw == (Word)~0ull && j0 + KT - 1 <= tl.hi0 &&
-                                                        (j0 >= tl.lo1 || j0 + KT <= a.sinks));
-        // A value that only some rows see meets the others' probability 0, which
-        // hides it unless it is not finite: such an element counts as 0 in the
-        // product and is added afterwards to the rows that see it.
-        int odd = 0;
-        if (!all) {
-#pragma unroll
-            for (int i = 0; i < TB / 16 / NTH; i++) {
-                uint4 x = ((uint4 *)vt)[tid + NTH * i];
-                const bool y[4] = {W::clean(x.x), W::clean(x.y), W::clean(x.z), W::clean(x.w)};
-                if (y[0] || y[1] || y[2] || y[3]) {
-                    odd = 1;
-                    ((uint4 *)vt)[tid + NTH * i] = x;
-                }
-            }
-            odd = __syncthreads_or(odd);
-        }
-        if (j0 > whi1 || (j0 + KT <= wlo0 && j0 >= a.sinks)) return;   // no row of this wave sees any
-        const bool every = __builtin_amdgcn_readfirstlane(okw == (Word)~0ull && j0 + KT - 1 <= whi0 &&
-                                                          (j0 >= wlo1 || j0 + KT <= a.sinks));
+        const bool every = whole(okw, j0, whi0, wlo1);
         wv.tile(kt, vt, ka, va, o, [&](int n, f16v &s, float sc) {
             if (!every) {
                 const uint32_t mine = (uint32_t)(okw >> (32 * n + 4 * hf));
@@ -420,22 +442,85 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         }
     };
 
+    if (t.nseq > 64) __syncthreads();   // (find_tile's words lie in k0)
     if (e0 < e1) {
-        copy(e0, page_of(e0), k0, v0, valid[0]);
+        const auto landed = [] { __builtin_amdgcn_s_waitcnt(0x0f70); };   // vmcnt(0): this wave's copies
+        uint64_t ok = copy(e0, page_of(e0), k0, v0);
         int pg = page_of(e0 + 1);
-        for (int e = e0;; e += 2) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's copies
-            __syncthreads();
-            if (e + 1 < e1) copy(e + 1, pg, k1, v1, valid[1]);
-            pg = page_of(e + 2);
-            tile(e, k0, v0, valid[0]);
-            if (e + 1 >= e1) break;
-            __builtin_amdgcn_s_waitcnt(0x0f70);
-            __syncthreads();
-            if (e + 2 < e1) copy(e + 2, pg, k0, v0, valid[0]);
-            pg = page_of(e + 3);
-            tile(e + 1, k1, v1, valid[1]);
-            if (e + 2 >= e1) break;
+        if constexpr (F32) {
+            constexpr int GR = DK / 8;   // groups of eight elements in a row
+            for (int e = e0; e < e1; e++) {
+                landed();
+                __syncthreads();
+                const bool all = whole(ok, tl.sp.block(e) * KT, tl.hi0, tl.lo1);
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < KT * GR / NTH; i++) {
+                    const int row = (tid + NTH * i) / GR, gr = (tid + NTH * i) % GR;
+                    const int to = row * W::ROW + (gr ^ W::swz(row)) * 16;
+                    float x[8];
+                    auto get = [&](const uint8_t *from) {
+                        *(f4 *)&x[0] = *(const f4 *)(from + row * ROW + gr * 32);
+                        *(f4 *)&x[4] = *(const f4 *)(from + row * ROW + gr * 32 + 16);
+                    };
+                    get(k0);
+                    W::put(x, kp + to);
+                    get(v0);
+                    if (!all)
+#pragma unroll
+                        for (int y = 0; y < 8; y++) odd |= W::clean(x[y]);
+                    W::put(x, vp + to);
+                }
+                if (!all) {   // a word of this wave's own rows, which it has read, says what it found
+                    odd = __any(odd);
+                    if (lane == 0) *(int *)(v0 + (64 * w) / GR * ROW) = odd;
+                }
+                __syncthreads();
+                if (!all) {
+                    odd = false;
+#pragma unroll
+                    for (int i = 0; i < NW; i++) odd |= *(const int *)(v0 + (64 * i) / GR * ROW) != 0;
+                    __syncthreads();
+                }
+                const uint64_t now = ok;
+                if (e + 1 < e1) ok = copy(e + 1, pg, k0, v0);
+                pg = page_of(e + 2);
+                tile(e, now, kp, vp, odd);
+            }
+        } else {
+            // cleaned in place where it has to be, and the products
+            auto turn = [&](int e, uint64_t now, const uint8_t *kt, uint8_t *vt) {
+                int odd = 0;
+                if (!whole(now, tl.sp.block(e) * KT, tl.hi0, tl.lo1)) {
+#pragma unroll
+                    for (int i = 0; i < TB / 16 / NTH; i++) {
+                        uint4 x = ((uint4 *)vt)[tid + NTH * i];
+                        const bool y[4] = {W::clean(x.x), W::clean(x.y), W::clean(x.z), W::clean(x.w)};
+                        if (y[0] || y[1] || y[2] || y[3]) {
+                            odd = 1;
+                            ((uint4 *)vt)[tid + NTH * i] = x;
+                        }
+                    }
+                    odd = __syncthreads_or(odd);
+                }
+                tile(e, now, kt, vt, odd != 0);
+            };
+            for (int e = e0;; e += 2) {
+                landed();
+                __syncthreads();
+                uint64_t now = ok;
+                if (e + 1 < e1) ok = copy(e + 1, pg, k1, v1);
+                pg = page_of(e + 2);
+                turn(e, now, k0, v0);
+                if (e + 1 >= e1) break;
+                landed();
+                __syncthreads();
+                now = ok;
+                if (e + 2 < e1) ok = copy(e + 2, pg, k0, v0);
+                pg = page_of(e + 3);
+                turn(e + 1, now, k1, v1);
+                if (e + 2 >= e1) break;
+            }
         }
     }
     l += __shfl_xor(l, 32, 64);
@@ -448,20 +533,11 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         ml[0] = m;
         ml[1] = l;
     }
-    // runs of four features: of one context tile's elements (16 bits), or across the tiles
-    if constexpr (sizeof(T) == 2 || DT == 2) {
 #pragma unroll
-        for (int d = 0; d < (sizeof(T) == 2 ? DT : 1); d++)
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int x = 0; x < 16; x += sizeof(T) == 2 ? 4 : 2) {
-                const f4 u = sizeof(T) == 2 ? f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}
-                                            : f4{o[0][x], o[DT / 2][x], o[0][x + 1], o[DT / 2][x + 1]};
-                *(f4 *)(op + W::feature(d, x, hf)) = u * f;
-            }
-    } else {
-#pragma unroll
-        for (int x = 0; x < 16; x++) *(f4 *)(op + W::feature(0, x, hf)) = f4{o[0][x], o[1][x], o[2][x], o[3][x]} * f;
-    }
+        for (int x = 0; x < 16; x += 4)
+            *(f4 *)(op + W::feature(d, x, hf)) = f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]} * f;
 }
 
 // The chunks of a tile's rows, joined in their order, as k_kv_join.
@@ -471,8 +547,9 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
     int at = blockIdx.x;
     const int h = at % A.t.Hk;
     at /= A.t.Hk;
+    __shared__ int lds[NW + 2];
     int b, rt;
-    if (!find_tile(A.t, A.a, at, b, rt)) return;
+    if (!find_tile(A.t, A.a, at, lds, b, rt)) return;
     const KvTile tl = kv_tile<RT, KB<T>>(A.t, A.a, b, rt);
     const int nch = (tl.sp.cnt + A.ct - 1) / A.ct, row = blockIdx.y * RB + threadIdx.x / LN;
     if (nch <= 1 || row >= tl.live) return;
@@ -544,15 +621,14 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const 
 
 }  // namespace
 
-// More rows of a sequence and K/V head than two tiles of the few-rows form hold (which reads the
-// keys once a tile): 16 requests of 2000 keys, 32 heads on 8, f16, 32 rows 51 us there and 48 here,
-// 48 rows 70 and 52; two of 30000 81 and 88, 115 and 92. f32 caches, on whose MFMA this form pays for its
-// idle rows, from four tiles: 8 heads, 40 rows 113 and 160, 64 rows 150 and 166.
-bool mh_kv_prompt(int type, const KvAttend &a) { return (int64_t)a.max_new * a.G > (type == KV_F32 ? 64 : 32); }
+// More rows of a sequence and K/V head than the few-rows form takes in one tile. Measured there
+// (tiles of 16 side by side) and here: two requests of 30000 keys, 32 heads on 8, f16, 48 rows 115
+// and 85 us, 64 of 1000 keys 154 and 81; f32, 16 requests of 2000 keys, 8 heads, 40 rows 113 and 99.
+bool mh_kv_prompt(const KvAttend &a) { return (int64_t)a.max_new * a.G > 32; }
 
 int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
     const Plan p = plan_of(nseq, rows, Hk, page, max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
-    if (p.wgs >= 1 << 30) return -1;
+    if (p.wgs >= 1 << 24) return -1;   // (a launch holds less than 2^32 threads)
     return p.nch > 1 ? p.wgs * RT * (dk + 2) : 0;
 }
 

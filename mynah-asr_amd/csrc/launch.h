@@ -237,6 +237,6 @@ struct KvAttend {
 int64_t mh_kv_attention_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &p);
 hipError_t mh_launch_kv_attention(const KvTables &t, int type, int dk, const KvAttend &p, float *ws, hipStream_t st);
 // its form for many rows of a sequence (kv_prompt.hip): whether the call takes it, the same two for it
-bool mh_kv_prompt(int type, const KvAttend &p);
+bool mh_kv_prompt(const KvAttend &p);
 int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &p);
 hipError_t mh_launch_kv_prompt(const KvTables &t, int type, int dk, const KvAttend &p, float *ws, hipStream_t st);

@@ -328,8 +328,41 @@ def test_prompt_window(gpu, typ, window, sinks):
     Case(typ, 64, 4, 2, 16, [350, 40], [350, 460]).check(gpu, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("nseq", [2, 63, 64, 65, 256, 257, 600])
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_prompts_of_many_sequences(gpu, typ, nseq):
+    """The order in which prompts' tiles are taken: sequences of no row, of one tile, of several."""
+    say("many prompts", typ, nseq)
+    r = np.random.default_rng(nseq)
+    new = [int(x) for x in r.choice([0, 1, 5, 16, 17, 40], nseq)]
+    new[-1] = 0
+    new[nseq // 2] = 33
+    c = Case(typ, 64, 8, 1, 16, new, [n + int(o) for n, o in zip(new, r.integers(0, 9, nseq))], pad=3)
+    c.check(gpu)
+
+
+@pytest.mark.parametrize("typ,dk", [("f32", 128), ("f16", 128), ("bf16", 128), ("f32", 64), ("f16", 64), ("bf16", 64)])
+@pytest.mark.parametrize("new,old,window,sinks", [(40, 9000, 0, 0), (9, 9000, 0, 0), (130, 3000, 0, 0), (130, 3000, 700, 5)])
+def test_parts_of_long_prompts(gpu, typ, dk, new, old, window, sinks):
+    """New rows on long caches, split over the keys and joined, against the definition on the GPU in 64 bits."""
+    import torch
+    say("part", typ, dk, new, old, window)
+    n = new + old
+    c = Case(typ, dk, 6, 2, 48, [new], [n])
+    out = c.attend(gpu, window=window, sinks=sinks).view(new, 6, dk).double()
+    flat = lambda p: p[c.d_pages[0].long()].permute(1, 0, 2, 3).reshape(2, -1, dk)[:, :n].double()   # noqa: E731
+    k, v = flat(c.k_pool), flat(c.v_pool)
+    p = torch.arange(old, n, device="cuda")[:, None]
+    j = torch.arange(n, device="cuda")[None]
+    see = (j <= p) & ((j > p - window) | (j < sinks)) if window else j <= p
+    for h in range(6):
+        s = (c.q.view(new, 6, dk)[:, h].double() @ k[h // 3].T.contiguous() * dk ** -0.5).masked_fill(~see, -np.inf)
+        ref = torch.softmax(s, 1) @ v[h // 3]
+        assert ((out[:, h] - ref).norm() / ref.norm()).item() <= 2.0 ** -19
+
+
 @pytest.mark.parametrize("typ,dk", [("f32", 128), ("f16", 64), ("bf16", 128)])
-@pytest.mark.parametrize("new", [[1, 1], [4, 4], [70, 3]])
+@pytest.mark.parametrize("new", [[1, 1], [4, 4], [40, 3], [70, 3]])
 def test_not_causal(gpu, typ, dk, new):
     say("not causal", typ, dk, new)
     Case(typ, dk, 4, 4, 25, new, [200, 75]).check(gpu, causal=0)
@@ -387,7 +420,8 @@ SPECIAL = [float("nan"), float("inf"), -float("inf")]
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("new,window", [([1, 1], 0), ([1, 1], 50), ([3, 2], 0), ([3, 2], 50), ([90, 75], 0), ([90, 75], 50)])
+@pytest.mark.parametrize("new,window", [([1, 1], 0), ([1, 1], 50), ([3, 2], 0), ([3, 2], 50), ([9, 12], 0), ([16, 3], 50),
+                                        ([90, 75], 0), ([90, 75], 50)])
 def test_what_is_not_seen_changes_nothing(gpu, typ, new, window):
     """Slots behind a sequence's end, in its last page and in pages of no sequence: NaN and infinities there leave every
     bit as it was; so do huge finite ones."""
@@ -439,7 +473,7 @@ def test_only_rows_that_see_a_nan_have_it(gpu, typ, new, where):
                 assert a[new // 2:last, 2:].isnan().all()
 
 
-@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("new", [1, 12, 70])
 def test_special_queries(gpu, new):
     """A NaN in a head's q makes that head NaN and no other."""
     import torch
@@ -453,7 +487,7 @@ def test_special_queries(gpu, new):
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("new", [1, 80])
+@pytest.mark.parametrize("new", [1, 14, 80])
 def test_scores_of_all_sizes(gpu, typ, new):
     """Scores that differ by hundreds (one key takes all), that are all alike, rows of q from 2^-40 to 2^30, zero rows."""
     import torch
@@ -530,9 +564,9 @@ def test_pool_beyond_4_gib(gpu):
         torch.cuda.empty_cache()
 
 
-@pytest.mark.parametrize("new", [1, 4, 150])
+@pytest.mark.parametrize("new", [1, 4, 5, 8])
 def test_same_bits_alone_and_in_a_batch(gpu, new):
-    """A sequence's rows do not depend on the others of the call, nor a call on the ones before it."""
+    """A sequence's rows (up to 32 a K/V head) do not depend on the others of the call, nor a call on the ones before it."""
     import torch
     say("alone", new)
     lengths = [new + 3, new + 400, new + 1200]

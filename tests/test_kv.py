@@ -25,9 +25,9 @@ def batch(**kw):
 
 
 CACHES = [dict(type=1), dict(type=24), dict(n_pages=0), dict(n_pages=-1), dict(page_size=0), dict(n_kv_heads=0),
-          dict(head_dim=96), dict(head_dim=0), dict(k=0), dict(v=0), dict(k=PTR + 8), dict(v=PTR + 2),
+          dict(head_dim=96), dict(head_dim=0), dict(n_kv_heads=65537), dict(k=0), dict(v=0), dict(k=PTR + 8), dict(v=PTR + 2),
           dict(n_pages=2 ** 30, page_size=16)]
-BATCHES = [dict(nseq=-1), dict(nseq=65536), dict(rows=-1), dict(rows=2 ** 24 + 1), dict(max_pages=-1), dict(max_new=-1),
+BATCHES = [dict(nseq=-1), dict(nseq=65536), dict(rows=-1), dict(rows=2 ** 24), dict(max_pages=-1), dict(max_new=-1),
            dict(max_len=-1), dict(max_len=2 ** 30 + 1), dict(row_start=0), dict(len=0), dict(pages=0),
            dict(row_start=PTR + 1), dict(len=PTR + 2), dict(pages=PTR + 3)]
 
@@ -76,9 +76,11 @@ def test_attention_refuses_small_workspace(lib):
 
 
 def test_attention_refuses_too_many_workgroups(lib):
-    b = batch(nseq=65535, rows=2 ** 24, max_new=32, max_pages=2 ** 26, max_len=2 ** 30)
-    refused(attention, lib, None, b)
-    assert M.kv_attention_ws_bytes(lib, cache(), b, 4) == 0
+    for new in (16, 17, 2 ** 24 - 1):   # (two heads a K/V head: 32 rows, the most of the few-rows form)
+        b = batch(nseq=65535, rows=2 ** 24 - 1, max_new=new, max_pages=2 ** 26, max_len=2 ** 30)
+        c = cache(n_kv_heads=512, n_pages=1)
+        refused(attention, lib, c, b, n_heads=1024, ldq=65536, ldo=65536)
+        assert M.kv_attention_ws_bytes(lib, c, b, 1024) == 0
 
 
 @pytest.mark.parametrize("bad", [
