@@ -34,9 +34,10 @@ namespace {
 constexpr int NW = 4, NTH = 64 * NW;
 constexpr int KB = 64;      // keys of a block
 
-// Blocks a wave takes in one chunk of a tile that sees `cnt`: long lists have
-// longer chunks (fewer partial results to join).
-KV_HD int wave_blocks(int cnt) { return cnt <= 256 ? 1 : cnt <= 1024 ? 2 : 4; }
+// Blocks a wave takes in one chunk of a tile that sees `cnt`. Up to 512 keys are one
+// chunk: the join would cost more than its second block. Long lists have longer chunks
+// (fewer partial results to join).
+KV_HD int wave_blocks(int cnt) { return cnt <= NW ? 1 : cnt <= 2 * NW ? 2 : cnt <= 256 ? 1 : cnt <= 1024 ? 2 : 4; }
 KV_HD int chunk_blocks(int cnt) { return NW * wave_blocks(cnt); }
 KV_HD int chunks_of(int cnt) { return cnt <= 0 ? 1 : (cnt + chunk_blocks(cnt) - 1) / chunk_blocks(cnt); }
 
@@ -239,27 +240,33 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
     const int nch = chunks_of(tl.sp.cnt), e0 = ch * chunk_blocks(tl.sp.cnt);
     if (ch >= nch) return;
 
-    // This wave's blocks, in parts of NB tiles of 16 keys: a part's loads are all on
-    // their way before the first product (the first part's before q is looked at).
+    // This wave's blocks, in parts of NB tiles of 16 keys. The first part's loads are on
+    // their way before q is looked at; the next part's keys are loaded once the scores
+    // have let go of their registers, its values once the context has.
     const int e1 = min(e0 + chunk_blocks(tl.sp.cnt), tl.sp.cnt);
     const bool alike = tl.lo0 == tl.lo1 && tl.hi0 == tl.hi1;   // every row sees the same keys
     uint32_t kr[NB][NU][4], vr[NB][4][VB / 4];
     int j0 = 0;
     uint64_t some = 0, all = 0;   // of the block's keys, those that some row sees, and every row
+    auto page_of = [&](int e) {   // (past the last block: the last one's again)
+        const int j = min(tl.sp.block(min(e, e1 - 1)) * KB + lane, tl.hi1);
+        return t.pages[(size_t)b * t.max_pages + j / t.page];
+    };
+    int pg = 0;                   // of block e's keys
     auto look = [&](int e) {      // where the block's keys lie
         j0 = tl.sp.block(e) * KB;
-        const int jl = j0 + lane, jc = min(jl, tl.hi1), lp = jc / t.page;
-        const int pg = t.pages[(size_t)b * t.max_pages + lp];
+        const int jl = j0 + lane;
         const bool in = jl <= tl.hi1 && (unsigned)pg < (unsigned)t.n_pages;
         const bool seen = in && (jl >= tl.lo0 || jl < a.sinks);
         some = __ballot(seen);
         all = __ballot(in && jl <= tl.hi0 && (jl >= tl.lo1 || jl < a.sinks));
         wave_lds_order();   // the reads of the last block's slots
-        slots[w][lane] = seen ? ((uint32_t)pg * t.Hk + h) * t.page + (jc - lp * t.page) : KV_NONE;
+        slots[w][lane] = seen ? ((uint32_t)pg * t.Hk + h) * t.page + jl % t.page : KV_NONE;
         wave_lds_order();
+        pg = page_of(e + NW);
     };
     auto part = [&](uint64_t m, int n0) { return (uint32_t)(m >> (16 * n0)) & (uint32_t)((1ull << (16 * NB)) - 1); };
-    auto fetch = [&](int n0) {
+    auto fetch_k = [&](int n0) {
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             const uint32_t at_k = slots[w][16 * (n0 + n) + c];
@@ -267,6 +274,8 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
 #pragma unroll
             for (int u = 0; u < NU; u++) load_run<16>(kp + 4 * EL * u, kr[n][u]);
         }
+    };
+    auto fetch_v = [&](int n0) {
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll
@@ -290,8 +299,12 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
         }
     };
     int e = e0 + w, n0 = 0;
+    if (e < e1) pg = page_of(e);
     bool more = seek(e, n0);
-    if (more) fetch(n0);
+    if (more) {
+        fetch_k(n0);
+        fetch_v(n0);
+    }
 
     // this lane's query rows (one of each sixteen), times scale and log2(e)
     int lo[NR], hi[NR];
@@ -316,14 +329,20 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
         f4 s[NR][NB];
 #pragma unroll
         for (int i = 0; i < NR; i++) wv[i].scores(ql + 64 * W::QF * i, kr, s[i]);
+        const uint32_t m_some = part(some, n0), m_all = part(all, n0);
+        const int jp = j0 + 16 * n0;   // the part's first key
+        n0 += NB;
+        if (n0 == KB / 16) n0 = 0, e += NW;
+        more = seek(e, n0);
+        if (more) fetch_k(n0);
         bool odd = false;
-        if (part(all, n0) != part(~0ull, 0)) {
-            const uint32_t see = part(some, n0) >> (4 * g);
+        if (m_all != part(~0ull, 0)) {
+            const uint32_t see = m_some >> (4 * g);
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const int j = j0 + 16 * (n0 + n) + 4 * g + x;
+                    const int j = jp + 16 * n + 4 * g + x;
                     const bool in = see >> (16 * n + x) & 1;
 #pragma unroll
                     for (int i = 0; i < NR; i++)
@@ -364,11 +383,10 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
         }
         W::template context<NR>(vr, s, o);
         if (__any(odd)) {
-            for (int jj = 16 * n0; jj < 16 * (n0 + NB); jj++) {
-                const uint32_t at_v = slots[w][jj];
-                const int j = j0 + jj;
-                if (at_v == KV_NONE) continue;
-                const T *vp = (const T *)t.v + (size_t)at_v * DK;
+            for (int jj = 0; jj < 16 * NB; jj++) {
+                const int j = jp + jj;
+                if (!(m_some >> jj & 1)) continue;
+                const T *vp = (const T *)t.v + (size_t)kv_slot(t, b, j, h) * DK;
 #pragma unroll
                 for (int i = 0; i < NR; i++) {
                     if (j > hi[i] || (j < lo[i] && j >= a.sinks)) continue;
@@ -382,10 +400,7 @@ __global__ __launch_bounds__(NTH, NR == 1 ? 3 : 2) void k_kv_step(const StepArgs
                 }
             }
         }
-        n0 += NB;
-        if (n0 == KB / 16) n0 = 0, e += NW;
-        more = seek(e, n0);
-        if (more) fetch(n0);
+        if (more) fetch_v(n0);
     }
 
     // join the waves
