@@ -21,7 +21,8 @@
 //   (The 32x32x2 f32 MFMA takes 2.7 times as long: four prompts with a window of 512,
 //   8 heads, 214 us, now 128.)
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
-// is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + 8).
+// is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + TOP), TOP 8 for f16,
+// whose small probabilities would be subnormal without it, else 0.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -142,6 +143,7 @@ template <typename T, int DK> struct Ops {   // 16 bits
     using X = KvTerms<T>;
     typedef typename X::v8 v8;
     static constexpr int KS = DK / 16, DT = DK / 32, ROW = DK * 2;
+    static constexpr float TOP = X::N == 2 ? 8.0f : 0.0f;
     // K fragments of the next half are read ahead where q's terms leave the registers
     static constexpr bool AHEAD = X::N * KS <= 16;
     // of any 16 rows that follow each other one piece each, and of any four the four
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[d] *= al;
             }
-            const float sub = 8.0f - (m == -INFINITY ? 0.0f : m);
+            const float sub = W::TOP - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
             for (int x = 0; x < 16; x++) {
                 s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sc, sub));

@@ -32,11 +32,12 @@ template <> struct KvTerms<_Float16> {
         t[1] = __builtin_bit_cast(v8, uint4{l[0], l[1], l[2], l[3]});
     }
     // the exponent that brings a row's maximum to [2^13, 2^14), near the top of f16's
-    // range: the second term of what matters is then no subnormal
+    // range: the second term of what matters is then no subnormal. At most 120, so that its
+    // reciprocal is no subnormal either: smaller rows have scores of 0 all the same.
     static __device__ __forceinline__ int shift(float mx) {
         int e = 14;
         if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &e);
-        return 14 - e;
+        return min(14 - e, 120);
     }
 };
 template <> struct KvTerms<__bf16> {

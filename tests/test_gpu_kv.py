@@ -408,6 +408,42 @@ def test_bounds_hold(gpu, new):
             assert (a - z).abs().max() <= 1e-4
 
 
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [40, 70]])
+def test_more_keys_than_the_table_holds(gpu, new):
+    """len past max_pages * page_size, under max_len: the keys that the table has no page for are not seen."""
+    say("past the table", new)
+    c = Case("bf16", 64, 4, 2, 16, new, [n + 100 for n in new], max_len=1 << 20)
+    held = c.pages.shape[1] * 16
+    for length in ([held + 1, held], [held + 3, held + 900], [10 ** 6, 2 ** 30]):
+        c.length = length
+        c.pages[c.pages < 0] = 0
+        c.upload()
+        c.max_len = held       # (the oracle's list of keys; the call still has 2^20)
+        c.check(gpu)
+        c.max_len = 1 << 20
+
+
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [40, 70]])
+def test_rows_before_the_first(gpu, new):
+    """row_start that begins behind the buffers' first rows: those are left as they are."""
+    import torch
+    say("rows before the first", new)
+    c = Case("f16", 64, 4, 2, 16, new, [n + 50 for n in new], pad=3)
+    ref = c.attend(gpu)
+    q, k = c.q.clone(), c.k.clone()
+    c.q[3:], c.k[3:] = q[:-3], k[:-3]
+    c.starts = [x + 3 for x in c.starts]
+    c.upload()
+    out = c.attend(gpu)
+    assert (out[:3] == 7.25).all() and torch.equal(out[3:], ref[:-3])
+    got = torch.full_like(c.q, 7.25)
+    torch.cuda.synchronize()
+    M.kv_append_dev(gpu, c.cache, c.batch, None, c.q.data_ptr(), c.ldq, 4, got.data_ptr(), c.ldq, c.k.data_ptr(), c.ldk,
+                    c.v.data_ptr(), c.ldk)
+    torch.cuda.synchronize()
+    assert (got[:3] == 7.25).all() and torch.equal(got[3:], c.q[3:])
+
+
 def test_row_start_of_no_use(gpu):
     c = Case("bf16", 64, 4, 2, 16, [5, 4], [9, 120])
     for starts in ([9, 9, 9], [0, 0, 0], [-3, -3, -2], [5, 5, 5]):
@@ -501,13 +537,18 @@ def test_scores_of_all_sizes(gpu, typ, new):
     c.check(gpu, scale=2.0 ** -31)
     c.check(gpu, scale=-2.0 ** -31)
     c.check(gpu, scale=0.0)
+    # rows at the lower end of f32's range, subnormal ones among them: every score is 0 to f32, hidden keys stay hidden
+    c.q[:] = torch.randn(c.q.shape, generator=torch.Generator().manual_seed(7)).cuda()
+    c.q[0], c.q[-1] = c.q[0] * 2.0 ** -126 * 2.0 ** -16, c.q[-1] * 2.0 ** -124
+    c.check(gpu)
+    c.check(gpu, window=60, sinks=3)
 
 
 def test_values_of_all_sizes(gpu):
     """Value features from 2^-24 to 2^15 (f16), 2^-100 to 2^100 (bf16, f32), each feature held to its own size."""
     import torch
-    for typ, lo, hi in (("f16", -14, 12), ("bf16", -100, 100), ("f32", -100, 100)):
-        for new in (1, 70):
+    for typ, lo, hi in (("f16", -14, 12), ("bf16", -100, 100), ("f32", -100, 100), ("bf16", 0, 107), ("f32", 0, 107)):
+        for new in (1, 12, 70):
             say("values", typ, new)
             c = Case(typ, 64, 4, 2, 16, [new], [new + 150])
             f = torch.exp2(torch.linspace(lo, hi, 64).round()).cuda()
