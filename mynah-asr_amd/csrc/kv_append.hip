@@ -15,6 +15,10 @@
 // walks the heads.
 // The angle is formed in 64 bits, in turns, and its whole turns dropped there:
 // at position 2^17 an f32 product would be off by 2^-7 rad.
+//
+// What bounds it: memory (12 prompts, 8300 rows of 32 heads on 8 of 128, f16: 83 us, 418 MB
+// at 5.0 TB/s; a large copy takes 4.8), for few rows a chain of four round trips, the
+// first of which the row's own loads share (256 rows 4.9 us, 4 rows 3.4).
 #include <hip/hip_runtime.h>
 #include <math.h>
 

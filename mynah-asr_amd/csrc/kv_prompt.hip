@@ -23,6 +23,12 @@
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
 // is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + TOP), TOP 8 for f16,
 // whose small probabilities would be subnormal without it, else 0.
+//
+// What bounds it: the card's power. One prompt of 8192 rows, 32 heads on 8 of 128, f16: 1015 to
+// 1040 us, 1.05 PFLOP/s of MFMAs issued (a large product of the library: 1.2); the same
+// on zeros 824. Without its softmax (234 VALU instructions a tile and wave to 64 MFMAs) it
+// takes 10% less, without its copies 11%. 32 rows a wave hold q's terms, the context and a
+// tile's fragments in 256 registers, two waves a SIMD.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
