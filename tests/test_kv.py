@@ -112,14 +112,14 @@ def test_valid_calls_get_as_far_as_the_device(lib):
 # ------------------------------------------------------------------- workspace
 def test_workspace_bytes(lib):
     c = cache(head_dim=128)
-    # up to 256 keys a sequence: one chunk, no partial results
-    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=256, max_pages=100), 4) == 0
-    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=257, max_pages=100), 4) > 0
+    # up to 512 keys a sequence: one chunk, no partial results
+    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=512, max_pages=100), 4) == 0
+    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=513, max_pages=100), 4) > 0
     # max_pages bounds the keys as well
-    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=257, max_pages=16), 4) == 0
+    assert M.kv_attention_ws_bytes(lib, c, batch(max_len=513, max_pages=32), 4) == 0
     # grows with every bound, never shrinks
     last = 0
-    for n in list(range(257, 20000, 61)) + [65536, 65600, 262144, 262208, 10 ** 6]:
+    for n in list(range(513, 20000, 61)) + [65536, 65600, 262144, 262208, 10 ** 6]:
         now = M.kv_attention_ws_bytes(lib, c, batch(max_len=n, max_pages=2 ** 20), 4)
         assert now >= last
         last = now
