@@ -28,7 +28,11 @@
 // 1040 us, 1.05 PFLOP/s of MFMAs issued (a large product of the library: 1.2); the same
 // on zeros 824. Without its softmax (234 VALU instructions a tile and wave to 64 MFMAs) it
 // takes 10% less, without its copies 11%. 32 rows a wave hold q's terms, the context and a
-// tile's fragments in 256 registers, two waves a SIMD.
+// tile's fragments in 256 registers, two waves a SIMD. Heads of 64 (eight bf16 prompts of
+// 100 to 4000 rows, 16 heads on 4) have half the MFMAs for a probability and are bound by the
+// VALU: 168 registers, three waves, 242 -> 232 us (f16, one prompt of 4096, 32 heads: 0.7%
+// slower). What a masked tile needs of a row is formed there (one bf16 prompt of 4096, 32 heads
+// of 128: 388 -> 374).
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -323,7 +327,7 @@ template <int DK> struct Ops<float, DK> : Ops<__bf16, DK> {
 };
 
 template <typename T, int DK>
-__global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
+__global__ __launch_bounds__(NTH, DK == 64 ? 3 : 2) void k_kv_prompt(const PromptArgs A) {
     using W = Ops<T, DK>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int DT = W::DT, KT = KB<T>;
@@ -351,17 +355,26 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
     if (ch >= nch) return;
     const int e0 = ch * A.ct, e1 = min(e0 + A.ct, tl.sp.cnt);
 
-    // this lane's row and its keys
-    const int r = 32 * w + c, tok = (rt * RT + min(r, tl.live - 1)) / a.G;
-    const int head = h * a.G + (rt * RT + min(r, tl.live - 1)) % a.G;
-    const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
+    // this lane's row: its token and head (formed where they are used: kept, they would cost registers
+    // that the products need)
+    auto row_of = [&](int &tok, int &head) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int r = rt * RT + min(32 * w + (ln & 31), tl.live - 1);
+        tok = r / a.G;
+        head = h * a.G + (r - tok * a.G);
+    };
     // what the wave's first and last row see (a wave of no rows: nothing)
     const bool idle = 32 * w >= tl.live;
     const int t0 = (rt * RT + min(32 * w, tl.live - 1)) / a.G, t1 = (rt * RT + min(32 * w + 31, tl.live - 1)) / a.G;
     const int wlo0 = kv_first(a, tl.s, t0), wlo1 = kv_first(a, tl.s, t1);
     const int whi0 = kv_last(t, a, tl.s, t0), whi1 = idle ? -1 : kv_last(t, a, tl.s, t1);
     W wv;
-    wv.init(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + head * DK, a.scale * 1.4426950408889634f, r < tl.live, lane);
+    {
+        int tok, head;
+        row_of(tok, head);
+        wv.init(a.q + (int64_t)(tl.s.r0 + tok) * a.ldq + head * DK, a.scale * 1.4426950408889634f, 32 * w + c < tl.live, lane);
+    }
     f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = zero16();
@@ -407,6 +420,9 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         const bool every = whole(okw, j0, whi0, wlo1);
         wv.tile(kt, vt, ka, va, o, [&](int n, f16v &s, float sc) {
             if (!every) {
+                int tok, head;
+                row_of(tok, head);
+                const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
                 const uint32_t mine = (uint32_t)(okw >> (32 * n + 4 * hf));
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
@@ -435,6 +451,9 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
             }
         });
         if (odd) {
+            int tok, head;
+            row_of(tok, head);
+            const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
             for (int jj = 0; jj < KT; jj++) {
                 const int j = j0 + jj;
                 if (!(okw >> jj & 1) || j > hi || (j < lo && j >= a.sinks)) continue;
@@ -532,7 +551,10 @@ __global__ __launch_bounds__(NTH, 2) void k_kv_prompt(const PromptArgs A) {
         }
     }
     l += __shfl_xor(l, 32, 64);
+    const int r = 32 * w + c;
     if (r >= tl.live) return;
+    int tok, head;
+    row_of(tok, head);
     const size_t slot = (size_t)blockIdx.x * RT + r;
     const float f = nch > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     float *op = nch > 1 ? A.part + slot * DK : a.out + (int64_t)(tl.s.r0 + tok) * a.ldo + head * DK;

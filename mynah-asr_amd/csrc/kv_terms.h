@@ -50,10 +50,12 @@ template <> struct KvTerms<__bf16> {
     static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
-    // x0, x1 rounded to a pair of bf16, and what that leaves of them
+    // x0, x1 rounded to a pair of bf16, and what that leaves of them (the pair kept from the compiler's
+    // sight: from conversions and their inverses it makes five instructions for each three)
     static __device__ __forceinline__ uint32_t pair(float &x0, float &x1) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        const uint32_t h = __builtin_bit_cast(uint32_t, b2{(__bf16)x0, (__bf16)x1});
+        uint32_t h = __builtin_bit_cast(uint32_t, b2{(__bf16)x0, (__bf16)x1});
+        asm("" : "+v"(h));
         x0 -= __uint_as_float(h << 16);
         x1 -= __uint_as_float(h & 0xffff0000u);
         return h;
