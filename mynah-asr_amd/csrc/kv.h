@@ -25,8 +25,9 @@ struct KvSeq {
     int r0, n, L;
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvTables &t, int b) {
-    const int r0 = max(t.row_start[b], 0), r1 = min(t.row_start[b + 1], t.rows);
-    return {r0, max(r1 - r0, 0), min(max(t.len[b], 0), 1 << 30)};
+    // (both within the rows before they are subtracted: 2^31 - 1 and -2^31 are 1 apart in 32 bits)
+    const int r0 = min(max(t.row_start[b], 0), t.rows), r1 = min(max(t.row_start[b + 1], r0), t.rows);
+    return {r0, r1 - r0, min(max(t.len[b], 0), 1 << 30)};
 }
 
 // Row of the pool (head_dim elements each) that holds key j of sequence b for

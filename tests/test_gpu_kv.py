@@ -452,6 +452,27 @@ def test_row_start_of_no_use(gpu):
         assert (c.attend(gpu) == 7.25).all()
 
 
+@pytest.mark.parametrize("new", [[5, 4], [40, 30], [1] * 70])
+def test_row_start_at_the_ends_of_its_type(gpu, new):
+    """2^31 - 1 before -2^31, whose difference is 1 in 32 bits, and the like: rows of no sequence stay as they are."""
+    import torch
+    low, high = -2 ** 31, 2 ** 31 - 1
+    n = len(new) + 1
+    c = Case("f16", 64, 4, 2, 16, new, [x + 70 for x in new])
+    before = c.k_pool.clone()
+    for first, rest in ((high, low), (high, low + 3), (high - 1, low), (low, low), (high, high), (c.rows, low)):
+        say("row_start", new, first, rest)
+        c.starts = [first] + [rest] * (n - 1)
+        c.upload()
+        assert (c.attend(gpu) == 7.25).all()
+        out = torch.full_like(c.q, 7.25)
+        torch.cuda.synchronize()
+        M.kv_append_dev(gpu, c.cache, c.batch, None, c.q.data_ptr(), c.ldq, 4, out.data_ptr(), c.ldq, c.k.data_ptr(),
+                        c.ldk, c.v.data_ptr(), c.ldk)
+        torch.cuda.synchronize()
+        assert (out == 7.25).all() and torch.equal(before, c.k_pool)
+
+
 SPECIAL = [float("nan"), float("inf"), -float("inf")]
 
 
