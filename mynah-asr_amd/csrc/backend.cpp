@@ -1158,18 +1158,23 @@ int kv_sizes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
     return 0;
 }
 
-// buf: 16-byte aligned, rows of `width` floats `ld` apart
-int kv_rows(const char *what, const float *buf, int64_t ld, int64_t width) {
-    if (!buf) return fail("bad argument: NULL", what);
+// buf: 16-byte aligned, n rows of `width` floats `ld` apart (n = 0: may be NULL)
+int kv_rows(const char *what, int n, const float *buf, int64_t ld, int64_t width) {
+    if (!buf && n > 0) return fail("bad argument: NULL", what);
     if ((uintptr_t)buf % 16 || ld % 4) return fail("rows must be 16-byte aligned, strides multiples of 4", what);
     if (ld < width || ld > (int64_t)1 << 32) return fail("row stride below the row's length, or above 2^32", what);
     return 0;
 }
 
+// (of no sequence there is none)
+bool kv_tables_missing(const mynah_asr_hip_kv_batch *b) {
+    return b->nseq > 0 && (!b->row_start || !b->len || (!b->pages && b->max_pages > 0));
+}
+
 int kv_pointers(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
     if (!c->k || !c->v || (uintptr_t)c->k % 16 || (uintptr_t)c->v % 16)
         return fail("bad argument: cache buffers must be there, 16-byte aligned");
-    if (!b->row_start || !b->len || (!b->pages && b->max_pages > 0)) return fail("bad argument: a NULL table of the batch");
+    if (kv_tables_missing(b)) return fail("bad argument: a NULL table of the batch");
     if ((uintptr_t)b->row_start % 4 || (uintptr_t)b->len % 4 || (uintptr_t)b->pages % 4)
         return fail("bad argument: a table of the batch is not 4-byte aligned");
     return 0;
@@ -1454,10 +1459,11 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
     const int dk = c->head_dim;
     if (n_heads < 0 || n_heads > 65536) return fail("n_heads must be 0 to 65536");
     if (!n_heads) q = nullptr, q_out = nullptr;
-    if (n_heads && (kv_rows("q", q, ldq, (int64_t)n_heads * dk) || kv_rows("q_out", q_out, ldqo, (int64_t)n_heads * dk)))
+    if (n_heads && (kv_rows("q", b->rows, q, ldq, (int64_t)n_heads * dk) || kv_rows("q_out", b->rows, q_out, ldqo, (int64_t)n_heads * dk)))
         return -1;
-    if (kv_rows("k", k, ldk, (int64_t)c->n_kv_heads * dk) || kv_rows("v", v, ldv, (int64_t)c->n_kv_heads * dk)) return -1;
-    if (n_heads && q_out == q && ldqo != ldq) return fail("q_out may be q with the same stride alone");
+    const int64_t kv_width = (int64_t)c->n_kv_heads * dk;
+    if (kv_rows("k", b->rows, k, ldk, kv_width) || kv_rows("v", b->rows, v, ldv, kv_width)) return -1;
+    if (q && q_out == q && ldqo != ldq) return fail("q_out may be q with the same stride alone");
     KvAppend a{};
     a.q = q, a.k = k, a.v = v, a.qo = q_out, a.ldq = ldq, a.ldqo = ldqo, a.ldk = ldk, a.ldv = ldv, a.Hq = n_heads;
     if (p) {
@@ -1497,8 +1503,8 @@ int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_
     t_err[0] = 0;
     if (kv_sizes(c, b) || kv_pointers(c, b) || kv_attend_sizes(c, n_heads, causal, window, sinks)) return -1;
     const int64_t width = (int64_t)n_heads * c->head_dim;
-    if (kv_rows("q", q, ldq, width) || kv_rows("out", out, ldo, width)) return -1;
-    if (out == q && ldo != ldq) return fail("out may be q with the same stride alone");
+    if (kv_rows("q", b->rows, q, ldq, width) || kv_rows("out", b->rows, out, ldo, width)) return -1;
+    if (q && out == q && ldo != ldq) return fail("out may be q with the same stride alone");
     if (!std::isfinite(scale)) return fail("scale must be finite");
     if ((uintptr_t)ws % 16) return fail("the workspace must be 16-byte aligned");
     KvAttend p = kv_attend(c, b, n_heads, causal, window, sinks);
@@ -1529,9 +1535,9 @@ int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_
 int mynah_asr_hip_kv_check(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b) {
     t_err[0] = 0;
     if (kv_sizes(c, b)) return -1;
-    if (!b->row_start || !b->len || (!b->pages && b->max_pages > 0)) return fail("bad argument: a NULL table of the batch");
+    if (kv_tables_missing(b)) return fail("bad argument: a NULL table of the batch");
     char at[64];
-    if (b->row_start[0] < 0) return fail("row_start[0] is negative");
+    if (b->nseq > 0 && b->row_start[0] < 0) return fail("row_start[0] is negative");
     std::vector<uint64_t> slots;   // of the new rows
     try {
         slots.reserve((size_t)b->rows);

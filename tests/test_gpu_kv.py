@@ -663,6 +663,11 @@ def test_empty_calls(gpu):
         setattr(c.batch, f, keep)
     c.batch.max_len = 0      # every key is past it
     assert (c.attend(gpu) == 0).all()
+    # no rows, or no sequences either: buffers of no bytes have no address
+    for b in (M.kv_batch(c.d_start.data_ptr(), c.d_len.data_ptr(), c.d_pages.data_ptr(), 1, 0, 1, 1, 16),
+              M.kv_batch(None, None, None, 0, 0, 0, 0, 0)):
+        M.kv_attention_dev(gpu, c.cache, b, None, c.ldq, 4, None, c.ldq, 0.125)
+        M.kv_append_dev(gpu, c.cache, b, None, None, c.ldq, 4, None, c.ldq, None, c.ldk, None, c.ldk)
 
 
 # ------------------------------------------------- streams, graphs, workspaces

@@ -107,6 +107,12 @@ def test_valid_calls_get_as_far_as_the_device(lib):
             call(lib)
     with pytest.raises(RuntimeError, match="no gfx950 device"):
         append(lib, n_heads=0, q=0, q_out=0)
+    # nothing to do, and an empty buffer has no address
+    for b in (batch(rows=0), batch(nseq=0, row_start=0, len=0, pages=0, rows=0)):
+        with pytest.raises(RuntimeError, match="no gfx950 device"):
+            attention(lib, b=b, q=0, out=0)
+        with pytest.raises(RuntimeError, match="no gfx950 device"):
+            append(lib, b=b, q=0, q_out=0, k=0, v=0)
 
 
 # ------------------------------------------------------------------- workspace
@@ -141,6 +147,7 @@ def tables(row_start, length, pages):
 def test_check_accepts(lib):
     M.kv_check(lib, cache(k=0, v=0), tables([0, 3, 3, 7], [20, 5, 4], [[1, 2], [2, 99], [3, -1]]))
     M.kv_check(lib, cache(), tables([0], [], np.zeros((0, 1))))
+    M.kv_check(lib, cache(), batch(nseq=0, row_start=0, len=0, pages=0))
 
 
 @pytest.mark.parametrize("row_start,length,pages,why", [
