@@ -30,7 +30,7 @@
 // takes 10% less, without its copies 11%. 32 rows a wave hold q's terms, the context and a
 // tile's fragments in 256 registers, two waves a SIMD. Heads of 64 (eight bf16 prompts of
 // 100 to 4000 rows, 16 heads on 4) have half the MFMAs for a probability and are bound by the
-// VALU: 168 registers, three waves, 242 -> 232 us (f16, one prompt of 4096, 32 heads: 0.7%
+// VALU: 168 registers, three waves, 242 -> 230 us (f16, one prompt of 4096, 32 heads: 0.7%
 // slower). What a masked tile needs of a row is formed there (one bf16 prompt of 4096, 32 heads
 // of 128: 388 -> 374).
 #include <hip/hip_runtime.h>
