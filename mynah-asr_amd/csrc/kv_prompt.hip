@@ -616,15 +616,21 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
     *(f4 *)(A.a.out + (int64_t)(tl.s.r0 + rr / A.a.G) * A.a.ldo + (h * A.a.G + rr % A.a.G) * DK + d) = o * inv;
 }
 
-// The launch's sizes, from the call's. A tile's keys are split into chunks (of 2
-// tiles at least) where its row tiles alone would leave the chip's 512 places
-// (two workgroups a CU) empty.
+// The launch's sizes, from the call's. A tile's keys are split into chunks where that is
+// likely to be faster: the longest chunk's tiles, one workgroup a CU or two, and the join of
+// the partial results, which grows with the workgroups (units of 0.1 us, measured). 64-row prompts
+// on 64 k keys, 8 heads of 128, f16, unsplit and in as many chunks as 512 places take: 32 of them,
+// k = 3, 17 and 26 us, k = 10 32 and 38, k = 40 98 and 94; four of them, k = 3, 14 and 15, k = 6 20
+// and 16, k = 40 27 in 8 chunks and 32 in 14.
 struct Plan {
     int ntile, nch, ct;
     int64_t wgs;
 };
-Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const KvAttend &a) {
+Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int type, const KvAttend &a) {
     Plan p;
+    const int kb = type == KV_F32 ? KB<float> : KB<__bf16>;
+    const int64_t one = type == KV_F32 ? 41 : type == KV_F16 ? 22 : 30;    // a tile, one workgroup a CU
+    const int64_t two = type == KV_F32 ? 41 : type == KV_F16 ? 36 : 48;    // two
     const int64_t per = ((int64_t)a.max_new * a.G + RT - 1) / RT;
     const int64_t most = ((int64_t)rows * a.G + RT - 1) / RT + nseq;
     const int64_t ntile = nseq * per < most ? nseq * per : most;
@@ -638,14 +644,17 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const 
         if (win + sink < blocks) blocks = win + sink;
     }
     if (blocks < 1) blocks = 1;
-    int64_t split = 512 / (ntile * Hk);
-    if (split < 1) split = 1;
-    int64_t ct = (blocks + split - 1) / split;
-    if (ct < 2) ct = 2;
+    const int64_t wgs = ntile * Hk;
+    int64_t ct = blocks, best = INT64_MAX;
+    for (int64_t n = 1; n == 1 || (n * wgs <= 512 && 2 * n <= blocks + 1); n += 1 + n / 8) {
+        const int64_t c = (blocks + n - 1) / n, w = (blocks + c - 1) / c * wgs;
+        const int64_t cost = c * (w <= 256 ? one : two) + (c < blocks ? 25 + w * 27 / 200 : 0);
+        if (cost < best) best = cost, ct = c;
+    }
     p.ntile = ntile < 1 << 30 ? (int)ntile : 1 << 30;
     p.ct = (int)ct;
     p.nch = (int)((blocks + ct - 1) / ct);
-    p.wgs = ntile * p.nch * Hk;
+    p.wgs = wgs * p.nch;
     return p;
 }
 
@@ -657,13 +666,13 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int kb, const 
 bool mh_kv_prompt(const KvAttend &a) { return (int64_t)a.max_new * a.G > 32; }
 
 int64_t mh_kv_prompt_ws(int nseq, int rows, int Hk, int page, int max_pages, int type, int dk, const KvAttend &a) {
-    const Plan p = plan_of(nseq, rows, Hk, page, max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
+    const Plan p = plan_of(nseq, rows, Hk, page, max_pages, type, a);
     if (p.wgs >= 1 << 24) return -1;   // (a launch holds less than 2^32 threads)
     return p.nch > 1 ? p.wgs * RT * (dk + 2) : 0;
 }
 
 hipError_t mh_launch_kv_prompt(const KvTables &t, int type, int dk, const KvAttend &a, float *ws, hipStream_t st) {
-    const Plan p = plan_of(t.nseq, t.rows, t.Hk, t.page, t.max_pages, type == KV_F32 ? KB<float> : KB<__bf16>, a);
+    const Plan p = plan_of(t.nseq, t.rows, t.Hk, t.page, t.max_pages, type, a);
     const PromptArgs A{t, a, ws, p.ntile, p.nch, p.ct};
     auto go = [&](auto step, auto join) {
         hipLaunchKernelGGL(step, dim3((unsigned)p.wgs), dim3(NTH), 0, st, A);
