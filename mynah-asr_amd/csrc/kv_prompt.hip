@@ -621,7 +621,7 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
 // the partial results, which grows with the workgroups (units of 0.1 us, measured). 64-row prompts
 // on 64 k keys, 8 heads of 128, f16, unsplit and in as many chunks as 512 places take: 32 of them,
 // k = 3, 17 and 26 us, k = 10 32 and 38, k = 40 98 and 94; four of them, k = 3, 14 and 15, k = 6 20
-// and 16, k = 40 27 in 8 chunks and 32 in 14.
+// and 16, k = 40 27 in 8 chunks and 32 in 14. f32, 32 of them on 192 keys 29 and 35.
 struct Plan {
     int ntile, nch, ct;
     int64_t wgs;
@@ -629,7 +629,7 @@ struct Plan {
 Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int type, const KvAttend &a) {
     Plan p;
     const int kb = type == KV_F32 ? KB<float> : KB<__bf16>;
-    const int64_t one = type == KV_F32 ? 41 : type == KV_F16 ? 22 : 30;    // a tile, one workgroup a CU
+    const int64_t one = type == KV_F16 ? 22 : 30;                          // a tile, one workgroup a CU
     const int64_t two = type == KV_F32 ? 41 : type == KV_F16 ? 36 : 48;    // two
     const int64_t per = ((int64_t)a.max_new * a.G + RT - 1) / RT;
     const int64_t most = ((int64_t)rows * a.G + RT - 1) / RT + nseq;
