@@ -443,7 +443,10 @@ int mynah_asr_hip_kv_attention_dev(const mynah_asr_hip_kv_cache *c, const mynah_
                                    int64_t ldq, int n_heads, float *out, int64_t ldo, float scale, int causal,
                                    int window, int sinks, void *ws, size_t ws_bytes, void *stream);
 /* Workspace bytes of that call, from its sizes alone (0: it needs none, or its
- * arguments are refused; the pointers of c and b are not looked at). */
+ * arguments are refused; the pointers of c and b are not looked at). Up to 32 rows
+ * (max_new * n_heads / n_kv_heads) a call of larger sizes needs no less; past that a
+ * smaller call may need more than a larger one, but none more than 262144
+ * (head_dim + 2) bytes. */
 size_t mynah_asr_hip_kv_attention_ws_bytes(const mynah_asr_hip_kv_cache *c, const mynah_asr_hip_kv_batch *b,
                                            int n_heads, int causal, int window, int sinks);
 /* Looks over a batch whose three tables are host memory (no GPU is used; the

@@ -135,6 +135,24 @@ def test_workspace_bytes(lib):
         assert M.kv_attention_ws_bytes(lib, c, b, 4) == 0
 
 
+@pytest.mark.parametrize("typ", [M.F32, M.F16, M.BF16])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_prompt_workspace_is_bounded(lib, typ, dk):
+    """Past 32 rows: never more than 512 workgroups' partial results of 128 rows; none where those alone fill the chip."""
+    c, most = cache(type=typ, head_dim=dk), 0
+    for nseq in (1, 2, 5, 31, 32, 200):
+        for new in (33, 128, 500, 4000):
+            for length in (new, 700, 5000, 100000, 2 ** 20):
+                for window in (0, 300):
+                    b = batch(nseq=nseq, rows=nseq * new, max_new=new, max_len=max(length, new), max_pages=2 ** 16)
+                    n = M.kv_attention_ws_bytes(lib, c, b, 2, 1, window, 0)
+                    assert n <= 262144 * (dk + 2) and n % (128 * 4 * (dk + 2)) == 0
+                    if 2 * nseq * -(-new // 128) > 256:
+                        assert n == 0
+                    most = max(most, n)
+    assert most > 0
+
+
 # -------------------------------------------------------------------- kv_check
 def tables(row_start, length, pages):
     t = [np.ascontiguousarray(x, np.int32) for x in (row_start, length, pages)]
