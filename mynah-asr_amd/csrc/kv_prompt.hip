@@ -629,8 +629,8 @@ struct Plan {
 Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int type, const KvAttend &a) {
     Plan p;
     const int kb = type == KV_F32 ? KB<float> : KB<__bf16>;
-    const int64_t one = type == KV_F16 ? 22 : 30;                          // a tile, one workgroup a CU
-    const int64_t two = type == KV_F32 ? 41 : type == KV_F16 ? 36 : 48;    // two
+    const int64_t one = type == KV_F32 ? 34 : type == KV_F16 ? 22 : 30;    // a tile, one workgroup a CU
+    const int64_t two = type == KV_F32 ? 45 : type == KV_F16 ? 36 : 48;    // two
     const int64_t per = ((int64_t)a.max_new * a.G + RT - 1) / RT;
     const int64_t most = ((int64_t)rows * a.G + RT - 1) / RT + nseq;
     const int64_t ntile = nseq * per < most ? nseq * per : most;
