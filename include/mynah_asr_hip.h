@@ -426,8 +426,9 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
  *
  * Products and sums as f32 ones: for finite inputs, and n max|v| below 2^120 over
  * the n keys a row sees, |out - ref| <= 2^-24 max|v| (2 (head_dim + 8) A + n / 8 +
- * 300), A the largest sum of |scale q k| over those keys (a bound; the relative
- * error measures 5e-7 to 1.2e-6). A row's bits
+ * 400), A the largest sum of |scale q k| over those keys (a bound; the relative
+ * error measures 4e-7 to 1.2e-6, up to 6e-6 where a prompt's keys and values are all
+ * alike). A row's bits
  * depend on its q, the keys and values it sees, its position, its place among its
  * sequence's new rows and their number, and the call's sizes and settings; up to 32
  * rows (max_new * n_heads / n_kv_heads), not on nseq either. Keys and values that it

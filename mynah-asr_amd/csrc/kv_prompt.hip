@@ -19,10 +19,15 @@
 //   each); six of the nine products of terms, all but those below 2^-24 of the whole.
 //   The copies of the next tile run into the one f32 slot while the planes are in use.
 //   (The 32x32x2 f32 MFMA takes 2.7 times as long: four prompts with a window of 512,
-//   8 heads, 214 us, now 128.)
+//   8 heads, 214 us, then 128.)
 // Statistics, in powers of two: a row's reference m follows its maximum only when that
 // is 2^6 above it, so the context is seldom rescaled; p = 2^(s - m + TOP), TOP 8 for f16,
 // whose small probabilities would be subnormal without it, else 0.
+// Sums: over thousands of keys that score alike, the roundings of one long f32 sum go the same way (relative
+// error 3e-5 at 8k keys, 1e-4 at 32k). So a tile's probabilities are summed as a tree, and each FOLD tiles
+// apart: the chains are at most 128 steps (l) and 512 (o), then one for each part. The whole's context waits
+// in the rows of the result (or the partial result): one prompt of 8192, f16, 64 tiles a part 1%, 32 3%; of
+// as many parts, eight ragged bf16 prompts, heads of 64, 1%.
 //
 // What bounds it: the card's power. One prompt of 8192 rows, 32 heads on 8 of 128, f16: 1015 to
 // 1040 us, 1.05 PFLOP/s of MFMAs issued (a large product of the library: 1.2); the same
@@ -48,6 +53,9 @@ namespace {
 constexpr int NW = 4, NTH = 64 * NW;
 constexpr int RT = 32 * NW;   // rows of a tile
 template <typename T> constexpr int KB = sizeof(T) == 4 ? 32 : 64;   // keys of a tile
+// Tiles that are summed before they join the whole (even). MFMAs that follow each other into one sum:
+// 8 a tile for f16, 12 for bf16 and f32.
+template <typename T> constexpr int FOLD = std::is_same_v<T, _Float16> ? 64 : 32;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -380,6 +388,55 @@ __global__ __launch_bounds__(NTH, DK == 64 ? 3 : 2) void k_kv_prompt(const Promp
     for (int d = 0; d < DT; d++) o[d] = zero16();
     float m = -INFINITY, l = 0.0f;
 
+    // Every FOLD<T> tiles o and l join the whole's context and sum, and start anew. The whole's
+    // context lies where the result will: the rows are this wave's own, and their q has
+    // been read. Its reference and sum: kept in registers, these two would push others out.
+    // (always_inline: of what a call does not inline, o lies in memory.)
+    volatile float whole_m, whole_l;
+    const bool split = nch > 1;
+    auto row_out = [&]() __attribute__((always_inline)) {
+        int tok, head;
+        row_of(tok, head);
+        return split ? A.part + ((size_t)blockIdx.x * RT + 32 * w + c) * DK
+                     : a.out + (int64_t)(tl.s.r0 + tok) * a.ldo + head * DK;
+    };
+    auto add_whole = [&](const float *op) __attribute__((always_inline)) {   // to o and l
+        const float mw = whole_m, al = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+        l += whole_l * al;
+#pragma unroll
+        for (int d0 = 0; d0 < DT; d0 += 2) {
+            f4 u[2][4];   // (on their way before the first is used)
+#pragma unroll
+            for (int d = 0; d < 2; d++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) u[d][x] = *(const f4 *)(op + W::feature(d0 + d, 4 * x, hf));
+#pragma unroll
+            for (int d = 0; d < 2; d++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[d0 + d][x] += u[d][x / 4][x % 4] * al;
+        }
+    };
+    auto put = [&](float *op, float f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int x = 0; x < 16; x += 4)
+                *(f4 *)(op + W::feature(d, x, hf)) = f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]} * f;
+    };
+    auto fold = [&](int e) __attribute__((always_inline)) {   // after tile e, the last of a part but not of all
+        if ((e + 1 - e0) % FOLD<T> || e + 1 == e1) return;
+        if (32 * w + c < tl.live) {
+            float *op = row_out();
+            if (e + 1 - e0 > FOLD<T>) add_whole(op);
+            put(op, 1.0f);
+        }
+        whole_m = m;
+        whole_l = l;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = zero16();
+    };
+
     // A lane holds the page of one row of a tile, read from the table a tile ahead and
     // looked at when it is used; wave w copies rows WR w .. of it.
     auto page_of = [&](int e) {
@@ -444,13 +501,14 @@ __global__ __launch_bounds__(NTH, DK == 64 ? 3 : 2) void k_kv_prompt(const Promp
                 for (int d = 0; d < DT; d++) o[d] *= al;
             }
             const float sub = W::TOP - (m == -INFINITY ? 0.0f : m);
+            float sum[8];   // (as a tree: l takes one step for 16 keys)
 #pragma unroll
-            for (int x = 0; x < 16; x++) {
-                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sc, sub));
-                l += s[x];
-            }
+            for (int x = 0; x < 16; x++) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sc, sub));
+#pragma unroll
+            for (int x = 0; x < 8; x++) sum[x] = s[2 * x] + s[2 * x + 1];
+            l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         });
-        if (odd) {
+        if (__builtin_expect(odd, 0)) {   // (as likely as not, it would take registers from the products: 3 to 9% slower)
             int tok, head;
             row_of(tok, head);
             const int lo = kv_first(a, tl.s, tok), hi = kv_last(t, a, tl.s, tok);
@@ -513,6 +571,7 @@ __global__ __launch_bounds__(NTH, DK == 64 ? 3 : 2) void k_kv_prompt(const Promp
                 if (e + 1 < e1) ok = copy(e + 1, pg, k0, v0);
                 pg = page_of(e + 2);
                 tile(e, now, kp, vp, odd);
+                fold(e);
             }
         } else {
             // cleaned in place where it has to be, and the products
@@ -547,27 +606,21 @@ __global__ __launch_bounds__(NTH, DK == 64 ? 3 : 2) void k_kv_prompt(const Promp
                 pg = page_of(e + 3);
                 turn(e + 1, now, k1, v1);
                 if (e + 2 >= e1) break;
+                fold(e + 1);
             }
         }
     }
-    l += __shfl_xor(l, 32, 64);
     const int r = 32 * w + c;
     if (r >= tl.live) return;
-    int tok, head;
-    row_of(tok, head);
-    const size_t slot = (size_t)blockIdx.x * RT + r;
-    const float f = nch > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    float *op = nch > 1 ? A.part + slot * DK : a.out + (int64_t)(tl.s.r0 + tok) * a.ldo + head * DK;
-    if (nch > 1 && hf == 0) {
-        float *ml = A.part + (size_t)gridDim.x * RT * DK + 2 * slot;
+    float *op = row_out();
+    if (e1 - e0 > FOLD<T>) add_whole(op);
+    l += __shfl_xor(l, 32, 64);
+    if (split && hf == 0) {
+        float *ml = A.part + (size_t)gridDim.x * RT * DK + 2 * ((size_t)blockIdx.x * RT + r);
         ml[0] = m;
         ml[1] = l;
     }
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int x = 0; x < 16; x += 4)
-            *(f4 *)(op + W::feature(d, x, hf)) = f4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]} * f;
+    put(op, split ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
 }
 
 // The chunks of a tile's rows, joined in their order, as k_kv_join.

@@ -831,3 +831,118 @@ def test_prompts_then_tokens(gpu, typ, window, sinks):
         assert np.linalg.norm(y - ref) <= 5e-6 * np.linalg.norm(ref)
     for w in dev.values():
         w.close()
+
+
+# ------------------------------------ long sums: prompts' keys in one workgroup
+# Forty sequences of 33 rows, eight heads: 320 workgroups, more than the chip has CUs, so no tile's keys are split and one
+# workgroup's sums reach over all of them.
+LONG = [("f32", 128), ("f16", 128), ("bf16", 128), ("f32", 64), ("f16", 64), ("bf16", 64)]
+
+
+def long_case(typ, dk, n, kind, nseq=40, new=33):
+    """All sequences on the same n keys. kind: random; plateau (the first 64 keys' scores 0, all others one score, 0.7 to 5
+    powers of two above them); alike (a plateau whose values are all the same, as frames of silence are)."""
+    import torch
+    c = Case(typ, dk, 8, 8, 64, [new] * nseq, [n] + [1] * (nseq - 1), seed=n, pad=1)
+    c.length, c.pages, c.max_len = [n] * nseq, c.pages[:1].expand(nseq, -1).contiguous(), n
+    if kind != "random":
+        first = c.pages[0, 0].item()
+        c.k_pool[:] = 0.5
+        c.k_pool[first] = 0.0
+        level = torch.linspace(1.0, 7.0, c.rows, device="cuda")[:, None] / dk ** 0.5     # q . k / sqrt(dk) = 0.5 to 3.5
+        c.q.mul_(0.01).add_(level)
+        if kind == "alike":
+            c.v_pool[:] = c.v_pool[:1, :, :1].clone()
+    c.upload()
+    return c
+
+
+def definition(c, window=0, sinks=0):
+    """[rows, heads, dim] in 64 bits: every sequence's rows over the keys of the first one's pages."""
+    import torch
+    n, dk, G = c.length[0], c.dk, c.heads // c.kv_heads
+    flat = lambda p: p[c.d_pages[0].long()].permute(1, 0, 2, 3).reshape(c.kv_heads, -1, dk)[:, :n].double()   # noqa: E731
+    k, v = flat(c.k_pool), flat(c.v_pool)
+    r = torch.arange(c.real, device="cuda")
+    start = torch.tensor(c.starts, device="cuda")
+    seq = torch.bucketize(r, start[1:], right=True)
+    p = (n - (start[seq + 1] - start[seq]) + r - start[seq])[:, None]
+    j = torch.arange(n, device="cuda")[None]
+    hidden = (j > p) | ((j <= p - window) & (j >= sinks)) if window else j > p
+    out = torch.empty(c.real, c.heads, dk, dtype=torch.float64, device="cuda")
+    for h in range(c.heads):
+        s = c.heads_of(c.q, c.heads)[:c.real, h].double() @ k[h // G].T.contiguous() * dk ** -0.5
+        out[:, h] = torch.softmax(s.masked_fill_(hidden, -np.inf), 1) @ v[h // G]
+    return out
+
+
+@pytest.mark.parametrize("n", [8200, 32700])
+@pytest.mark.parametrize("kind", ["random", "plateau", "alike"])
+@pytest.mark.parametrize("typ,dk", LONG)
+def test_long_sums(gpu, typ, dk, kind, n):
+    """The sums of probabilities and of values over thousands of keys. Independent roundings: the norm's bar, as above.
+    Values all alike: the output is that value whatever the scores are, and roundings of a sum may all go one way, so each
+    of the sum's steps counts. A part of 64 tiles (f16; else 32) takes 8 (12) a tile into the context, two into the sum of
+    probabilities and 4 that sum a tile's; the parts, 1024 keys at least, n / 1024 each; 16 are for the exponential, the
+    terms, the reciprocal and its product."""
+    say("long sums", typ, dk, kind, n)
+    c = long_case(typ, dk, n, kind)
+    out = c.attend(gpu)
+    assert (out[c.real:] == 7.25).all()
+    y, ref = c.heads_of(out, 8)[:c.real].double(), definition(c)
+    rel = ((y - ref).norm() / ref.norm()).item()
+    worst = ((y - ref).abs() / ref.abs()).max().item() / U
+    say(f"  norm {rel:.3g}, worst {worst:.4g} u")
+    if kind == "alike":
+        assert worst <= (64 * 10 if typ == "f16" else 32 * 14) + 20 + n / 512
+    else:
+        assert rel <= 2.0 ** -19
+
+
+@pytest.mark.parametrize("n", [1024, 1057, 2047, 2048, 2049, 4096, 4129, 8192, 8225, 9000])
+@pytest.mark.parametrize("typ,dk", LONG)
+def test_long_sums_in_parts(gpu, typ, dk, n):
+    """Lengths around the ends of parts, with and without a window; out in place of q."""
+    import torch
+    for window, sinks in ((0, 0), (n - 700, 70)):
+        say("parts", typ, dk, n, window)
+        c = long_case(typ, dk, n, "random")
+        out = c.attend(gpu, window=window, sinks=sinks)
+        assert (out[c.real:] == 7.25).all()
+        y, ref = c.heads_of(out, 8)[:c.real].double(), definition(c, window, sinks)
+        assert ((y - ref).norm() / ref.norm()).item() <= 2.0 ** -19
+        c.attend(gpu, window=window, sinks=sinks, out=c.q)
+        assert torch.equal(c.q[:c.real], out[:c.real])
+
+
+@pytest.mark.parametrize("typ,dk", LONG)
+def test_long_sums_of_split_keys(gpu, typ, dk):
+    """A prompt's part on a long cache in eight chunks (64 workgroups a chunk), each longer than a part of its sums."""
+    say("split", typ, dk)
+    c = Case(typ, dk, 8, 8, 64, [1000], [30000])
+    y, ref = c.heads_of(c.attend(gpu), 8).double(), definition(c)
+    assert M.kv_attention_ws_bytes(gpu, c.cache, c.batch, 8) == 512 * 128 * 4 * (dk + 2)
+    assert ((y - ref).norm() / ref.norm()).item() <= 2.0 ** -19
+
+
+@pytest.mark.parametrize("typ,dk", LONG)
+def test_long_sums_keep_a_nan_where_it_is(gpu, typ, dk):
+    """A value that is not finite, in the first part of the sums, the second, or the last rows' own: its feature alone, of the
+    rows that see it."""
+    import torch
+    n = 9000
+    c = long_case(typ, dk, n, "random")
+    base = c.attend(gpu).view(c.rows, 8, dk)
+    for j in (100, 5000, n - 10):
+        for bad in SPECIAL:
+            say("nan", typ, dk, j, bad)
+            at = int(c.pages[0, j // 64]), 3, j % 64, 5
+            keep = c.v_pool[at].clone()
+            c.v_pool[at] = bad
+            out = c.attend(gpu).view(c.rows, 8, dk)
+            c.v_pool[at] = keep
+            sees = torch.zeros(c.rows, dtype=torch.bool, device="cuda")
+            sees[:c.real] = torch.arange(c.real, device="cuda") % 33 + n - 33 >= j
+            assert not out[sees, 3, 5].isfinite().any()
+            out[sees, 3, 5] = base[sees, 3, 5]
+            assert torch.equal(out, base)
