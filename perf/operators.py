@@ -135,7 +135,12 @@ def _lengths(case):
 
 # ----------------------------------------------------------------- the inputs
 def prepare(case, seed):
-    """What a serving loop holds before the call: the cache, the batch's tables and the rows of q, k and v."""
+    """What a serving loop holds before the call: the cache, the batch's tables and the rows of q, k and v. With `own` on the
+    default stream, the current stream becomes one that the framework can be given, as a program sets it up once: inputs,
+    calls and what reads their outputs are then in order without waits."""
+    if own and not torch.cuda.current_stream().cuda_stream:
+        _framework()
+        torch.cuda.set_stream(_stream)
     g = torch.Generator(device="cuda").manual_seed(seed)
     dt, hq, hk, dk, page = TYPES[case["type"]], case["heads"], case["kv_heads"], case["dim"], case["page"]
     lengths = _lengths(case)
@@ -203,16 +208,36 @@ def _framework():
         sys.path.insert(0, at)
     import mynah_hip as M
     if _lib is None:
-        _lib, _stream = M.HipLib(), torch.cuda.Stream()   # one stream: a thread's calls share its workspace
+        _lib, _stream = M.HipLib(), torch.cuda.Stream()
     return M
+
+
+def _current(device):
+    """The handle of the current stream (what torch.cuda.current_stream(device).cuda_stream gives, which takes 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _on_a_stream(s, call):
+    """call(handle) in the order of the caller's current stream. The framework takes 0, the handle of torch's default
+    stream, for the thread's own stream; from there the call goes by a stream between two waits."""
+    handle = _current(s["device"])
+    if handle:
+        call(handle)
+        return
+    here = torch.cuda.current_stream(s["device"])
+    _stream.wait_stream(here)
+    call(_stream.cuda_stream)
+    here.wait_stream(_stream)
 
 
 def _handles(s):
     """The descriptions of the cache and the batch that a program makes once."""
     M = _framework()
     c = s["case"]
-    h = {"M": M, "cache": M.kv_cache({"f32": M.F32, "f16": M.F16, "bf16": M.BF16}[c["type"]], s["k_cache"].data_ptr(),
-                                     s["v_cache"].data_ptr(), s["n_pages"], s["page"], s["kv_heads"], s["dim"]),
+    kind = {"f32": M.F32, "f16": M.F16, "bf16": M.BF16}[c["type"]]
+    h = {"M": M, "device": s["q"].device.index,
+         "cache": M.kv_cache(kind, s["k_cache"].data_ptr(), s["v_cache"].data_ptr(), s["n_pages"], s["page"], s["kv_heads"],
+                             s["dim"]),
          "batch": M.kv_batch(s["row_start"].data_ptr(), s["len"].data_ptr(), s["pages"].data_ptr(), c["nseq"], s["rows"],
                              s["pages"].shape[1], s["max_new"], s["max_len"])}
     if c["op"] == "append":
@@ -223,17 +248,17 @@ def _handles(s):
 
 
 def _append_own(s):
-    s["M"].kv_append_dev(_lib, s["cache"], s["batch"], s["prep"], s["q"].data_ptr(), s["q"].stride(0), s["heads"],
-                         s["q_out"].data_ptr(), s["q_out"].stride(0), s["k"].data_ptr(), s["k"].stride(0),
-                         s["v"].data_ptr(), s["v"].stride(0), _stream.cuda_stream)
+    _on_a_stream(s, lambda stream: s["M"].kv_append_dev(
+        _lib, s["cache"], s["batch"], s["prep"], s["q"].data_ptr(), s["q"].stride(0), s["heads"], s["q_out"].data_ptr(),
+        s["q_out"].stride(0), s["k"].data_ptr(), s["k"].stride(0), s["v"].data_ptr(), s["v"].stride(0), stream))
     return {"q": s["q_out"], "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
 
 
 def _attention_own(s):
     c = s["case"]
-    s["M"].kv_attention_dev(_lib, s["cache"], s["batch"], s["q"].data_ptr(), s["q"].stride(0), s["heads"],
-                            s["out"].data_ptr(), s["out"].stride(0), s["scale"], int(c["causal"]), c["window"], c["sinks"],
-                            stream=_stream.cuda_stream)
+    _on_a_stream(s, lambda stream: s["M"].kv_attention_dev(
+        _lib, s["cache"], s["batch"], s["q"].data_ptr(), s["q"].stride(0), s["heads"], s["out"].data_ptr(),
+        s["out"].stride(0), s["scale"], int(c["causal"]), c["window"], c["sinks"], stream=stream))
     return s["out"]
 
 
