@@ -424,11 +424,14 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
  * n_heads heads, ldq / ldo floats apart, 16-byte aligned, strides multiples of
  * 4; out may be q (ldo = ldq), and may not overlap it otherwise.
  *
- * Products and sums as f32 ones: for finite inputs, and n max|v| below 2^120 over
- * the n keys a row sees, |out - ref| <= 2^-24 max|v| (2 (head_dim + 8) A + n / 8 +
- * 400), A the largest sum of |scale q k| over those keys (a bound; the relative
- * error measures 4e-7 to 1.2e-6, up to 6e-6 where a prompt's keys and values are all
- * alike). A row's bits
+ * Products and sums as f32 ones: over the n keys a row sees, |out - ref| <= 2^-24
+ * max|v| (2 (head_dim + 8) A + n / 8 + 400), A the largest sum of |scale q k| over
+ * those keys (a bound; the relative error measures 4e-7 to 1.2e-6, up to 6e-6 where a
+ * prompt's keys and values are all alike). In A an element of q counts as no less than
+ * 2^-20 of its head's largest for f16 caches; for bf16 and f32 ones, scale q and k as no
+ * less than 2^-100. That holds for finite inputs with scale and max|v| 0 or from 2^-100
+ * in size, scale, scale q and A up to 2^100 and n max|v| below 2^120; past that a row may
+ * be off by more, or NaN. A row's bits
  * depend on its q, the keys and values it sees, its position, its place among its
  * sequence's new rows and their number, and the call's sizes and settings; up to 32
  * rows (max_new * n_heads / n_kv_heads), not on nseq either. Keys and values that it

@@ -946,3 +946,55 @@ def test_long_sums_keep_a_nan_where_it_is(gpu, typ, dk):
             assert not out[sees, 3, 5].isfinite().any()
             out[sees, 3, 5] = base[sees, 3, 5]
             assert torch.equal(out, base)
+
+
+# --------------------------------------------- the range that the bound is for
+def bound_of(c, scale):
+    """What the header allows each row and head, with its floors under the elements of q and k (in float64)."""
+    q, k = np.abs(f64(c.heads_of(c.q, c.heads))), np.abs(f64(c.k_pool))
+    if c.typ == "f16":
+        q = np.maximum(q, 2.0 ** -20 * q.max(-1, keepdims=True))
+    else:
+        q, k = np.maximum(q, 2.0 ** -100 / abs(scale)), np.maximum(k, 2.0 ** -100)
+    _, terms, count, vmax = (x[:c.real] for x in O.attention(k, f64(c.v_pool), c.starts, c.length, c.pages.numpy(), q, scale))
+    return U * vmax * (2 * (c.dk + 8) * terms + count / 8 + 400)
+
+
+RANGES = {"wide rows": ["f16"], "small q": ["bf16", "f32"], "large q": ["bf16", "f32"], "small scale": ["f16", "bf16", "f32"],
+          "large scale": ["f16", "bf16", "f32"], "largest q": ["f16", "bf16", "f32"], "smallest v": ["bf16", "f32"]}
+
+
+@pytest.mark.parametrize("new", [1, 12, 70])
+@pytest.mark.parametrize("kind,typ", [(k, t) for k, ts in RANGES.items() for t in ts])
+def test_range_of_the_bound(gpu, typ, kind, new):
+    """Scores of order 1 from elements at the ends of what the header's bound is stated for."""
+    say("range", kind, typ, new)
+    c = Case(typ, 64, 4, 2, 16, [new], [new + 90])
+    scale = 0.125
+    if kind == "wide rows":        # one feature 2^24 times the others; the keys have nothing there
+        c.q.mul_(8)
+        c.q[:, ::64] *= 2.0 ** 24
+        c.k_pool[..., 0] = 0
+    elif kind == "small q":        # |scale q| of 2^-95
+        c.q.mul_(2.0 ** -92)
+        c.k_pool.mul_(2.0 ** 95)
+    elif kind == "large q":
+        c.q.mul_(2.0 ** 95)
+        c.k_pool.mul_(2.0 ** -92)
+    elif kind == "small scale":    # the sizes of q that make up for it
+        scale = 2.0 ** -100
+        c.q.mul_(2.0 ** 97)
+    elif kind == "large scale":
+        scale = 2.0 ** 100
+        c.q.mul_(2.0 ** -103)
+    elif kind == "largest q":      # on keys that have nothing: the values' mean
+        c.q.clamp_(-4, 4).mul_(2.0 ** 100)
+        c.k_pool.zero_()
+    else:
+        c.v_pool.mul_(2.0 ** -100)
+    y = f64(c.heads_of(c.attend(gpu, scale), 4))[:c.real]
+    ref = O.attention(f64(c.k_pool), f64(c.v_pool), c.starts, c.length, c.pages.numpy(), f64(c.heads_of(c.q, 4)), scale)[0]
+    err = np.abs(y - ref[:c.real]).max(-1)
+    lim = bound_of(c, scale)
+    say(f"  worst {(err / lim).max():.3g} of the bound")
+    assert np.isfinite(y).all() and (err <= lim).all()
