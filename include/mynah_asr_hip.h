@@ -431,13 +431,14 @@ int mynah_asr_hip_kv_append_dev(const mynah_asr_hip_kv_cache *c, const mynah_asr
  * 2^-20 of its head's largest for f16 caches; for bf16 and f32 ones, scale q and k as no
  * less than 2^-100. That holds for finite inputs with scale and max|v| 0 or from 2^-100
  * in size, scale, scale q and A up to 2^100 and n max|v| below 2^120; past that a row may
- * be off by more, or NaN. A row's bits
- * depend on its q, the keys and values it sees, its position, its place among its
+ * be off by more, or NaN. A row's bits depend on its q, the keys and values it sees, its position, its place among its
  * sequence's new rows and their number, and the call's sizes and settings; up to 32
  * rows (max_new * n_heads / n_kv_heads), not on nseq either. Keys and values that it
  * does not see (hidden, behind len[b], in the rest of a page) change nothing, NaN
- * and infinity included. A row that sees a NaN or an infinity gives what f32
- * arithmetic gives or NaN: a key's in the whole head, a value's in its feature alone.
+ * and infinity included. A row that sees a NaN gives NaN; one that sees an infinity NaN
+ * or what f32 arithmetic gives, but it may give 0 where all its scores are -infinity, and
+ * keep a value's infinity whose probability has become 0. A key's reach the whole head, a
+ * value's its feature alone.
  *
  * ws: device workspace of ws_bytes, 16-byte aligned, at least
  * mynah_asr_hip_kv_attention_ws_bytes; NULL: the calling thread's own, grown as

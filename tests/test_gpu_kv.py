@@ -998,3 +998,33 @@ def test_range_of_the_bound(gpu, typ, kind, new):
     lim = bound_of(c, scale)
     say(f"  worst {(err / lim).max():.3g} of the bound")
     assert np.isfinite(y).all() and (err <= lim).all()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 12, 70])
+def test_infinite_scores(gpu, typ, new):
+    """Keys of -infinity under positive queries: of a row that sees others too, they take nothing or make it NaN; a row
+    that sees nothing else is 0 or NaN, never a value. Of +infinity: NaN."""
+    import torch
+    say("infinite scores", typ, new)
+    c = Case(typ, 64, 4, 2, 16, [new], [new + 40])
+    c.q.abs_().add_(0.01)
+    c.v_pool.abs_().add_(1.0)
+    c.k_pool[:] = -float("inf")
+    y = c.attend(gpu)
+    assert ((y == 0) | y.isnan()).all()
+    first = c.pages[0, 0].item()
+    c.k_pool[first] = 0.5
+    base = c.attend(gpu, causal=0)
+    held = c.length
+    c.length, c.starts = [16], [0, min(new, 16)]         # the same rows on the finite keys alone
+    c.upload()
+    few = c.attend(gpu, causal=0)[:min(new, 16)]
+    c.length, c.starts = held, [0, new]
+    c.upload()
+    got = base[:min(new, 16)]
+    size = 0.125 * 0.5 * c.heads_of(c.q, 4).sum(-1).max().item()      # the header's A; each of the two is within its bound
+    lim = 2 * U * c.v_pool.max().item() * (2 * 72 * size + 16 / 8 + 400)
+    assert (got.isnan() | ((got - few).abs() <= lim)).all()
+    c.k_pool[first, :, 3] = float("inf")
+    assert c.attend(gpu, causal=0).isnan().all()
