@@ -390,7 +390,8 @@ typedef struct {
 } mynah_asr_hip_kv_batch;
 
 /* What the append does to the heads of q and k first. The norm of a head x:
- * x / sqrt(mean(x^2) + eps) * w (squares summed in 64 bits). Then the rotation of
+ * x / sqrt(mean(x^2) + eps) * w (squares summed in 64 bits; NaN throughout where an
+ * element of the head is not finite, or all are 0 and eps too). Then the rotation of
  * the first `rot` features at the row's position p: pair i becomes
  * (a cos t - b sin t, a sin t + b cos t), t = p * freq[i] (formed in 64 bits). */
 typedef struct {

@@ -101,10 +101,12 @@ __global__ __launch_bounds__(NTH) void k_kv_append(const KvTables t, const KvApp
             }
 #pragma unroll
             for (int m = 1; m < TP; m *= 2) ss += __shfl_xor(ss, m, 64);
-            const float r = (float)rsqrt_d(ss / DK + (double)a.eps);
+            const double rd = rsqrt_d(ss / DK + (double)a.eps);
+            // (without eps, the factor of subnormal elements passes f32's range: part of it goes first)
+            const float up = rd > 0x1p120 ? 0x1p64f : 1.0f, r = (float)(rd / up);
             const f4 w0 = *(const f4 *)(w + e0), w1 = *(const f4 *)(w + e1);
 #pragma unroll
-            for (int i = 0; i < 4; i++) x0[i] = x0[i] * r * w0[i], x1[i] = x1[i] * r * w1[i];
+            for (int i = 0; i < 4; i++) x0[i] = x0[i] * up * r * w0[i], x1[i] = x1[i] * up * r * w1[i];
         }
         if (!isv && l < a.rot / 8) {
             // pair i of this lane: (x0[i], x1[i]), or neighbours of x0 and x1

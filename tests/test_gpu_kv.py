@@ -1028,3 +1028,38 @@ def test_infinite_scores(gpu, typ, new):
     assert (got.isnan() | ((got - few).abs() <= lim)).all()
     c.k_pool[first, :, 3] = float("inf")
     assert c.attend(gpu, causal=0).isnan().all()
+
+
+# ---------------------------------------------------------- the append's edges
+@pytest.mark.parametrize("power", [-145, -140, -126, -60, 125])
+def test_append_norm_of_all_sizes(gpu, power):
+    """Heads of subnormal elements and of ones near f32's largest, without eps: the norm brings both to 1."""
+    say("norm", power)
+    c = Case("f32", 64, 4, 2, 16, [3, 5], [30, 5])
+    c.q.mul_(2.0 ** (power // 2)).mul_(2.0 ** (power - power // 2))
+    c.k.mul_(2.0 ** (power // 2)).mul_(2.0 ** (power - power // 2))
+    run_append(gpu, c, dict(preps(64)["both"], eps=0.0))
+
+
+def test_append_norm_of_what_is_not_finite(gpu):
+    """An infinity or a NaN makes its head NaN, and no other; so does a head of zeros without eps."""
+    import torch
+    prep = preps(64)["norm"]
+    qn, kn = (torch.from_numpy(prep[n]).cuda() for n in ("qn", "kn"))
+    p = M.kv_prep(qn.data_ptr(), kn.data_ptr(), 0.0)
+    c = Case("f32", 64, 4, 2, 16, [3], [3])
+    outs = []
+    for bad in [None] + SPECIAL + [0.0]:
+        q = c.q.clone()
+        if bad is not None:
+            q[1, 64 if bad == 0.0 else 70:128 if bad == 0.0 else 71] = bad
+        out = torch.full_like(q, 7.25)
+        torch.cuda.synchronize()
+        M.kv_append_dev(gpu, c.cache, c.batch, p, q.data_ptr(), c.ldq, 4, out.data_ptr(), c.ldq, c.k.data_ptr(), c.ldk,
+                        c.v.data_ptr(), c.ldk)
+        torch.cuda.synchronize()
+        if bad is not None:
+            assert out[1, 64:128].isnan().all()
+            out[1, 64:128] = outs[0][1, 64:128]
+        outs.append(out)
+        assert torch.equal(out, outs[0]) and out.isfinite().all()
