@@ -1063,3 +1063,45 @@ def test_append_norm_of_what_is_not_finite(gpu):
             out[1, 64:128] = outs[0][1, 64:128]
         outs.append(out)
         assert torch.equal(out, outs[0]) and out.isfinite().all()
+
+
+@pytest.mark.parametrize("typ,dk", LONG)
+@pytest.mark.parametrize("prep", ["norm", "both", "part", "inter"])
+def test_append_without_q_prepares_k(gpu, typ, dk, prep):
+    """n_heads 0 with a norm and a rotation of k: the bits that the whole call writes, which are right."""
+    import torch
+    say("append without q", typ, dk, prep)
+    c = Case(typ, dk, 6, 2, 7, [3, 0, 1, 12], [10, 5, 1, 12], pad=3, ldx=8)
+    pools = c.k_pool.clone(), c.v_pool.clone()
+    run_append(gpu, c, preps(dk)[prep])
+    whole = c.k_pool.clone(), c.v_pool.clone()
+    c.k_pool.copy_(pools[0])
+    c.v_pool.copy_(pools[1])
+    spec = preps(dk)[prep]
+    dev = {n: torch.from_numpy(np.asarray(spec[n])).cuda() for n in ("qn", "kn", "freq") if spec.get(n) is not None}
+    ptr = {n: dev[n].data_ptr() if n in dev else None for n in ("qn", "kn", "freq")}
+    p = M.kv_prep(ptr["qn"], ptr["kn"], spec.get("eps", 0.0), spec.get("rot", 0), spec.get("interleaved", False), ptr["freq"])
+    torch.cuda.synchronize()
+    M.kv_append_dev(gpu, c.cache, c.batch, p, None, 0, 0, None, 0, c.k.data_ptr(), c.ldk, c.v.data_ptr(), c.ldk)
+    torch.cuda.synchronize()
+    assert torch.equal(c.k_pool, whole[0]) and torch.equal(c.v_pool, whole[1])
+
+
+# ------------------------------------------------------------- mixed batches
+@pytest.mark.parametrize("typ,dk", LONG)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 5)])
+def test_prompts_and_tokens_in_one_call(gpu, typ, dk, window, sinks):
+    """A prompt, single tokens on long and short caches and a few rows: one form for all, its keys split over chunks that
+    the shorter sequences do not have."""
+    say("mixed", typ, dk, window)
+    c = Case(typ, dk, 8, 2, 16, [130, 1, 1, 0, 3], [130, 3000, 40, 7, 900], pad=2)
+    assert M.kv_attention_ws_bytes(gpu, c.cache, c.batch, 8, 1, window, sinks) > 0
+    c.check(gpu, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("typ,dk", LONG)
+def test_windowed_parts_of_several_sequences(gpu, typ, dk):
+    say("windowed parts", typ, dk)
+    c = Case(typ, dk, 2, 1, 25, [300, 200, 90], [2300, 1800, 90], pad=2)
+    assert M.kv_attention_ws_bytes(gpu, c.cache, c.batch, 2, 1, 700, 5) > 0
+    c.check(gpu, window=700, sinks=5)
