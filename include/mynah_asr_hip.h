@@ -375,7 +375,10 @@ typedef struct {
  * buffers: a key in a page outside [0, n_pages) is not written and not seen, nor
  * is a key at or past max_pages * page_size; for the attention, neither is one
  * at or past max_len, and rows of a sequence past its first max_new are left as
- * they are. A len below 0 counts as 0. With nseq 0 the tables may be NULL, with rows 0
+ * they are. max_new and max_len size the launch and the workspace, so a call costs more
+ * the further they lie above what the tables hold, and max_new chooses the attention's
+ * form for all the call's sequences: prompts and long sequences of single rows are faster
+ * in two calls. A len below 0 counts as 0. With nseq 0 the tables may be NULL, with rows 0
  * the activations. mynah_asr_hip_kv_check looks host copies over. */
 typedef struct {
     int nseq;              /* sequences, up to 65535 */

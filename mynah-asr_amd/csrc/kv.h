@@ -1,5 +1,5 @@
-// kv.h — what the paged-cache kernels (kv_append.hip, kv_attention.hip) share:
-// the tables of a call, and which keys a row sees. Plain integer arithmetic,
+// kv.h — what the paged-cache kernels (kv_append.hip, kv_attention.hip, kv_prompt.hip)
+// share: the tables of a call, and which keys a row sees. Plain integer arithmetic,
 // for the host (workspace sizes) and the device.
 #pragma once
 #include <hip/hip_runtime.h>

@@ -26,18 +26,19 @@
 // Sums: over thousands of keys that score alike, the roundings of one long f32 sum go the same way (relative
 // error 3e-5 at 8k keys, 1e-4 at 32k). So a tile's probabilities are summed as a tree, and each FOLD tiles
 // apart: the chains are at most 128 steps (l) and 512 (o), then one for each part. The whole's context waits
-// in the rows of the result (or the partial result): one prompt of 8192, f16, 64 tiles a part 1%, 32 3%; of
-// as many parts, eight ragged bf16 prompts, heads of 64, 1%.
+// in the rows of the result (or the partial result). That costs 1% of one prompt of 8192 rows, f16 (with 32
+// tiles a part 4%), 1% of eight ragged bf16 prompts with heads of 64, 4% of one f32 prompt of 4096 with these.
 //
-// What bounds it: the card's power. One prompt of 8192 rows, 32 heads on 8 of 128, f16: 1015 to
-// 1040 us, 1.05 PFLOP/s of MFMAs issued (a large product of the library: 1.2); the same
-// on zeros 824. Without its softmax (234 VALU instructions a tile and wave to 64 MFMAs) it
-// takes 10% less, without its copies 11%. 32 rows a wave hold q's terms, the context and a
-// tile's fragments in 256 registers, two waves a SIMD. Heads of 64 (eight bf16 prompts of
-// 100 to 4000 rows, 16 heads on 4) have half the MFMAs for a probability and are bound by the
-// VALU: 168 registers, three waves, 242 -> 230 us (f16, one prompt of 4096, 32 heads: 0.7%
-// slower). What a masked tile needs of a row is formed there (one bf16 prompt of 4096, 32 heads
-// of 128: 388 -> 374).
+// What bounds it: the card's power. One prompt of 8192 rows, 32 heads on 8 of 128, f16: 1020 to
+// 1030 us, 1.05 PFLOP/s of MFMAs issued (a large product of the library: 1.2). As first built
+// (1042 us) it took 824 on zeros, 10% less without its softmax, 11% without its copies. 32 rows a
+// wave hold q's terms, the context and a tile's fragments in 256 registers, two waves a SIMD, and
+// not all fits: 3 to 20 vector registers a lane and some 90 to 170 scalar ones are spilled. One wave
+// a SIMD needs no spill and takes 11 to 19% longer on 16-bit caches (f32, one prompt of 4096, 8 heads: 7%
+// less; four with a window: 39% longer). Heads of 64 (eight bf16 prompts of 100 to 4000 rows, 16 heads on 4) have half
+// the MFMAs for a probability and are bound by the VALU: 168 registers, three waves, up to 4 spilled,
+// 242 -> 230 us then, now 234 (f16, one prompt of 4096, 32 heads: 0.7% slower). What a masked tile needs of a row is
+// formed there (one bf16 prompt of 4096, 32 heads of 128: 388 -> 374).
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -671,7 +672,9 @@ __global__ __launch_bounds__(NTH) void k_kv_prompt_join(const PromptArgs A) {
 
 // The launch's sizes, from the call's. A tile's keys are split into chunks where that is
 // likely to be faster: the longest chunk's tiles, one workgroup a CU or two, and the join of
-// the partial results, which grows with the workgroups (units of 0.1 us, measured). 64-row prompts
+// the partial results, which grows with the workgroups (units of 0.1 us, measured on heads of 128; heads of
+// 64, with half the work a tile and three workgroups a CU, go by the same). Every tile counts as long as
+// the longest may be, by max_len and the window. 64-row prompts
 // on 64 k keys, 8 heads of 128, f16, unsplit and in as many chunks as 512 places take: 32 of them,
 // k = 3, 17 and 26 us, k = 10 32 and 38, k = 40 98 and 94; four of them, k = 3, 14 and 15, k = 6 20
 // and 16, k = 40 27 in 8 chunks and 32 in 14. f32, 32 of them on 192 keys 29 and 35.
@@ -713,7 +716,9 @@ Plan plan_of(int nseq, int rows, int Hk, int page, int max_pages, int type, cons
 
 }  // namespace
 
-// More rows of a sequence and K/V head than the few-rows form takes in one tile. Measured there
+// More rows of a sequence and K/V head than the few-rows form takes in one tile. The whole call takes the
+// form of its longest sequence: of 60 single rows on 500 to 100000 keys (32 heads on 8, f16, 855 us) and a part
+// of 512 rows (25) in one call, 3060 us. Measured there
 // (tiles of 16 side by side) and here: two requests of 30000 keys, 32 heads on 8, f16, 48 rows 115
 // and 85 us, 64 of 1000 keys 154 and 81; f32, 16 requests of 2000 keys, 8 heads, 40 rows 113 and 99.
 bool mh_kv_prompt(const KvAttend &a) { return (int64_t)a.max_new * a.G > 32; }
